@@ -76,7 +76,7 @@ def lib():
             raise RuntimeError(f"{LIB_PATH} is missing: build it with `make -C detllm_b200/csrc` "
                                "(or __graft_entry__.build())")
         L = C.CDLL(LIB_PATH)
-        P, SZ, I, U32, U64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64
+        P, SZ, I, U32, U64, F32 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64, C.c_float
         sig = {
             "det_status_string": (C.c_char_p, [I]),
             "det_device_count": (I, [C.POINTER(I)]),
@@ -109,6 +109,14 @@ def lib():
             "det_model_profile": (I, [P, C.c_char_p, SZ, I]),
             "det_session_gemv_stream": (I, [P, U32, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
             "det_symbol_ranges_noalloc": (I, [P, U32, U32, P, I, P, P]),
+            "det_token_scores": (I, [P, P, P, U32, U32, P, P, P, P]),
+            "det_distill_loss": (I, [P, P, U32, P, P, U32, F32, P]),
+            "det_token_scores_device": (I, [P, I, U32, U32, U64, P, I, U32, P, P, P, P, P, P, P]),
+            "det_token_scores_grad_device": (I, [P, I, U32, U32, U64, P, I, P, P, P, P, U64, P]),
+            "det_token_scores_step_device": (I, [P, I, U32, U32, U64, P, I, P, P, P, P, P, P, U64, P, P]),
+            "det_distill_loss_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P]),
+            "det_distill_grad_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, U64, P]),
+            "det_distill_step_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P, U64, P, P]),
             "det_tp_exchange_timeout_selftest": (I, [I]),
             "det_q6k_pipeline_timeout_selftest": (I, [I]),
             "det_add_latency_cycles": (I, [I, C.POINTER(C.c_double)]),
@@ -233,6 +241,42 @@ class Model:
     def session(self, n_ctx: int, max_chunk: int = 64) -> "Session":
         return Session(self, n_ctx, max_chunk)
 
+    def score(self, tokens, n_ctx: int = 0, top: int = 0):
+        """What ``compress`` pays for a token stream, before coding: per token
+        ``(logprob, entropy, top_ids, top_logprobs)`` under the codec's own
+        windows (``n_ctx`` 0 = model context, overlap ``n_ctx // 4``).
+        -logprob / ln 2 is the token's ideal code length in bits.  A token
+        without context (the first) is scored as uniform over the vocabulary,
+        with tokens 0, 1, ... as its alternatives."""
+        t = _u32(tokens)
+        if not 0 <= top <= min(128, self.vocab) or (t.size and int(t.max()) >= self.vocab):
+            raise ValueError("top must be in 0 .. 128 and at most the vocabulary, and tokens inside it")
+        n_ctx = n_ctx or self.config.context_length
+        if not 0 < n_ctx <= self.config.context_length:
+            raise ValueError("n_ctx must be in 1 .. the model's context length")
+        lp, en = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
+        ids, lps = np.empty((t.size, top), np.uint32), np.empty((t.size, top), np.float32)
+        if t.size == 0:
+            return lp, en, ids, lps
+        even = np.log(self.vocab)
+        overlap, start, i = n_ctx // 4, 0, 0
+        with Session(self, n_ctx, min(1024, n_ctx)) as s:
+            while i < t.size:  # a window: tokens i .. end - 1 are read in it
+                end = min(start + n_ctx, t.size)
+                if i == start:
+                    lp[i], en[i], ids[i], lps[i] = -even, even, np.arange(top), -even
+                for p in range(start, end - 1, s.max_chunk):
+                    q = min(p + s.max_chunk, end - 1)
+                    s.forward(t[p:q], p - start)
+                    first = max(p, i - 1)  # row j - p scores token j + 1
+                    if first < q:
+                        r = slice(first + 1, q + 1)
+                        lp[r], en[r], ids[r], lps[r] = s.token_scores(t[r], np.arange(first - p, q - p), top)
+                i, start = end, end - overlap
+                if i < t.size:
+                    s.reset()
+        return lp, en, ids, lps
+
     def encode_symbols(self, symbols, n_ctx: int, overlap: int, byte_escapes: bool = True) -> bytes:
         s = _u32(symbols)
         out, n = C.c_void_p(), C.c_size_t()
@@ -299,6 +343,39 @@ class Session:
         _check(lib().det_decoder_lookup(self._h, row, int(byte_escapes), value, C.byref(sym), C.byref(r)),
                "det_decoder_lookup")
         return sym.value, r.cum, r.freq, r.total
+
+    def token_scores(self, tokens, rows=None, top: int = 0):
+        """Of each row of the last forward (``rows``, else 0, 1, ...): the log
+        probability (natural) of its token, the entropy and the ``top`` (at
+        most 128) most likely tokens with their log probabilities, most likely
+        first: ``(logprob, entropy, top_ids, top_logprobs)``.  A token of
+        0xFFFFFFFF is ignored (log probability 0)."""
+        t = _u32(tokens)
+        r = _u32(rows) if rows is not None else None
+        if r is not None and r.size != t.size:
+            raise ValueError("rows and tokens must have the same length")
+        if top < 0:
+            raise ValueError("top must not be negative")
+        lp, en = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
+        ids, lps = np.empty((t.size, top), np.uint32), np.empty((t.size, top), np.float32)
+        _check(lib().det_token_scores(self._h, _ptr(r) if r is not None else None, _ptr(t), t.size, top, _ptr(lp),
+                                      _ptr(en), _ptr(ids), _ptr(lps)), "det_token_scores")
+        return lp, en, ids, lps
+
+    def distill_loss(self, teacher_ids, teacher_logits, rows=None, temperature: float = 1.0) -> np.ndarray:
+        """Divergence (natural) of each row of the last forward from a
+        teacher's list (``[n, k]`` tokens and logits or log probabilities, k
+        at most 128; an id of 0xFFFFFFFF is no entry): what coding with this
+        model costs beyond the teacher, over the listed tokens."""
+        i = np.ascontiguousarray(teacher_ids, dtype=np.uint32)
+        u = np.ascontiguousarray(teacher_logits, dtype=np.float32)
+        r = _u32(rows) if rows is not None else None
+        if i.ndim != 2 or i.shape != u.shape or (r is not None and r.size != i.shape[0]):
+            raise ValueError("teacher_ids and teacher_logits must be [n, k], and rows n")
+        loss = np.empty(i.shape[0], np.float32)
+        _check(lib().det_distill_loss(self._h, _ptr(r) if r is not None else None, i.shape[0], _ptr(i), _ptr(u),
+                                      i.shape[1], temperature, _ptr(loss)), "det_distill_loss")
+        return loss
 
     def gemv_stream(self, reps: int = 20):
         """(ms, bytes) per pass of the one-token weight GEMVs run back to back."""

@@ -277,6 +277,9 @@ struct det_session {
   det::RcState* h_rc = nullptr;
   uint32_t* d_row0 = nullptr;
   Graph graph_dev1;
+  // token scores and distillation (scoring.cu): device buffer and its pinned
+  // copy, allocated at first use
+  uint8_t *d_score = nullptr, *h_score = nullptr;
 };
 
 namespace det {

@@ -199,6 +199,14 @@ cudaError_t launch_cdf_prepare(const Launch& L, const float* logits, int V, cons
                                float* e, float* z);
 cudaError_t launch_cdf_ranges(const Launch& L, const float* e, const float* z, int V, int tail,
                               const uint32_t* rows, const uint32_t* symbols, int n, uint64_t* out3);
+// Token scores and distillation on a session's f32 logits (scoring.cu): row
+// rows[i] for output i.  tokens as int32 (negative: ignored); top list arrays
+// may be null when top is 0; lists are k entries, int32 ids and f32 values
+cudaError_t launch_token_scores(const Launch& L, const float* logits, int V, const uint32_t* rows,
+                                const uint32_t* tokens, int n, int top, float* logprob, float* entropy,
+                                int32_t* top_ids, float* top_logprobs);
+cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, const uint32_t* rows, int n,
+                                const int32_t* ids, const float* teacher, int k, float temperature, float* loss);
 cudaError_t launch_expf(cudaStream_t st, const float* x, float* y, long long n);
 // GGUF tensor bytes (in device memory) -> device layouts (repack.cu); a
 // non-finite scale or value sets ERRF_NONFINITE in *err

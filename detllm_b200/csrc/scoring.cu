@@ -1,0 +1,695 @@
+// scoring.cu -- what a row of logits says about tokens: the log probability
+// of a given token, the row's entropy and its most likely tokens, and how far
+// a student's row is from a teacher's top list; with the gradients of both.
+//
+//   m = max x, d_j = (x_j - m) / T, S = sum exp(d_j), S1 = sum exp(d_j) d_j
+//   log p_j = d_j - log S          H = log S - S1 / S
+//   loss = sum_i q_i (log q_i - log p_id(i)),  q = softmax(u / T)
+//   d log p_t / dx_j = [j = t] - p_j
+//   dH / dx_j        = -p_j (log p_j + H) = -p_j (d_j - S1 / S)
+//   d loss / dx_j    = (p_j - sum_{i: id(i) = j} q_i) / T
+//
+// An entry of -inf is masked out: exp(-inf) = 0 and 0 * -inf counts as 0.
+//
+// Arithmetic: every f32 operation is rounded on its own, as in the rest of
+// the library, and the order of every sum is fixed by the vocabulary alone,
+// so a row has the same bits whatever batch, stride or call it is part of.
+// A row is cut into segments of 2,048 entries; a warp takes a segment, its
+// lane l the entries of 16-byte vectors l, l + 32, ... of it, and sums are
+// relative to the segment's own maximum until the segments are joined.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "../../include/detgpu.h"
+#include "dev_math.cuh"
+#include "internal.h"
+
+namespace det {
+namespace {
+
+constexpr int kSeg = 2048;                       // entries per segment
+constexpr int kPerLane = kSeg / 32;              // entries per lane of a segment
+constexpr uint32_t kMaxVocab = 1u << 18;         // as the CDF's alphabet
+constexpr int kMaxSegs = (int)(kMaxVocab / kSeg);
+constexpr int kThreads = 256;
+constexpr uint32_t kFull = 0xffffffffu;
+
+// ---- packed f32 pairs ----------------------------------------------------------
+using f2 = unsigned long long;
+DI f2 pk(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+DI float2 un(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+DI f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+DI f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+DI f2 fma2(unsigned long long a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// c + p where p is a product: written p * 1 + c, which is exact in its
+// multiply and rounds once, like the add; `one` is 1.0 at run time, so the
+// compiler cannot contract the multiply that made p into the add.
+DI f2 addp(f2 p, f2 one, f2 c) { return fma2(p, one, c); }  // exact multiply
+
+DI float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// exp(d) for d <= 0, two at a time: d = k ln 2 + r with |r| <= ln 2 / 2 (a
+// two-part ln 2 whose parts times k are exact), exp(r) by a degree-5 minimax
+// polynomial 1 + r + r^2 q(r) (relative error 1.06e-7), 2^k added to the
+// exponent field.  Below kExpLow the result is +0 (the exponent field goes
+// negative there and the integer maximum clears it); it is within 3.1 * 2^-24
+// of exp(d) for d >= -87.  NaN gives an unspecified number: callers keep d,
+// which stays NaN, beside it.
+constexpr float kExpLow = -88.13f;  // k = -127, r = -0.10
+struct Exp2 {
+  f2 e, d;  // exp, and the argument as clamped
+};
+DI Exp2 exp2_lanes(f2 d, f2 one) {
+  float2 c = un(d);
+  c.x = max_nan(c.x, kExpLow);
+  c.y = max_nan(c.y, kExpLow);
+  d = pk(c.x, c.y);
+  const f2 magic = pk(12582912.0f, 12582912.0f), nmagic = pk(-12582912.0f, -12582912.0f);
+  const f2 z = addp(mul2(d, pk(1.44269504f, 1.44269504f)), one, magic);
+  const f2 k = add2(z, nmagic);
+  const f2 nhi = pk(-0.693145751953125f, -0.693145751953125f);
+  const f2 nlo = pk(-1.4286197256296873e-06f, -1.4286197256296873e-06f);
+  // k has 7 bits and the parts of ln 2 have 15: exact products
+  const f2 r = fma2(k, nlo, fma2(k, nhi, d));
+  f2 q = addp(mul2(pk(0.008312501f, 0.008312501f), r), one, pk(0.04189033f, 0.04189033f));
+  q = addp(mul2(q, r), one, pk(0.16667116f, 0.16667116f));
+  q = addp(mul2(q, r), one, pk(0.4999923f, 0.4999923f));
+  const f2 p = add2(addp(mul2(q, mul2(r, r)), one, r), pk(1.0f, 1.0f));
+  const float2 pf = un(p), zf = un(z);
+  const int ex = max(__float_as_int(pf.x) + (__float_as_int(zf.x) << 23), 0);
+  const int ey = max(__float_as_int(pf.y) + (__float_as_int(zf.y) << 23), 0);
+  return {pk(__int_as_float(ex), __int_as_float(ey)), d};
+}
+DI float exp1(float d, float one) { return un(exp2_lanes(pk(d, d), pk(one, one)).e).x; }
+
+// ---- element types ---------------------------------------------------------------
+template <typename T>
+DI float to_f32(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __half2float(v);
+  else return __bfloat162float(v);
+}
+template <typename T>
+DI T from_f32(float v) {  // one rounding, to nearest even
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+DI float load_any(const void* p, int dtype, size_t i) {
+  if (dtype == DET_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == DET_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+DI long long load_id(const void* p, int bytes, size_t i) {
+  return bytes == 8 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+}
+
+// ---- a segment -------------------------------------------------------------------
+// entry of lane l, vector i, element j of a segment
+template <typename T>
+DI int seg_entry(int l, int i, int j) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  return i * 32 * VEC + l * VEC + j;
+}
+
+struct Sums {
+  float m, s, s1;
+};
+
+DI float warp_max(float v) {
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+DI float warp_sum(float v) {
+  for (int o = 16; o > 0; o >>= 1) v = fadd(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+DI double warp_sum_d(double v) {
+  for (int o = 16; o > 0; o >>= 1) v = dadd(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
+// maximum, sum of exp((x - m) / T) and the same weighted by (x - m) / T over
+// one segment's 64 entries per lane; a NaN or +inf anywhere leaves s1 NaN
+DI Sums segment_sums(const float (&x)[kPerLane], float inv_t, float one_) {
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < kPerLane; i++) m = fmaxf(m, x[i]);
+  m = warp_max(m);
+  const float base = m == -INFINITY ? 0.0f : -m;
+  const f2 nm = pk(base, base), one = pk(one_, one_), it = pk(inv_t, inv_t);
+  f2 s[2] = {0, 0}, w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < kPerLane / 2; i++) {
+    const Exp2 e = exp2_lanes(mul2(add2(pk(x[2 * i], x[2 * i + 1]), nm), it), one);
+    s[i & 1] = add2(s[i & 1], e.e);
+    w[i & 1] = addp(mul2(e.e, e.d), one, w[i & 1]);
+  }
+  const float2 sp = un(add2(s[0], s[1])), wp = un(add2(w[0], w[1]));
+  return {m, warp_sum(fadd(sp.x, sp.y)), warp_sum(fadd(wp.x, wp.y))};
+}
+
+// joins a row's segments (one warp; the result in every lane)
+DI Sums join_segments(const float* sm, const float* ss, const float* sw, int nseg, float inv_t, float one) {
+  const int l = threadIdx.x & 31;
+  float m = -INFINITY;
+  for (int i = l; i < nseg; i += 32) m = fmaxf(m, sm[i]);
+  m = warp_max(m);
+  float s = 0.0f, w = 0.0f;
+  for (int i = l; i < nseg; i += 32) {
+    const bool empty = sm[i] == -INFINITY;
+    const float d = empty ? kExpLow : fmaxf(fmul(fsub(sm[i], m), inv_t), kExpLow);
+    const float f = exp1(d, one);
+    s = fadd(s, fmul(f, ss[i]));
+    // sum of exp(d_j + d) (d_j + d) = f (S1 + d S); NaN stays NaN
+    w = fadd(w, fmul(f, fadd(sw[i], fmul(d, ss[i]))));
+  }
+  return {m, warp_sum(s), warp_sum(w)};
+}
+
+struct RowStats {
+  float m, s, s1, log_s;
+  bool empty, bad;
+};
+DI RowStats finish_row(const Sums& r) {
+  RowStats t;
+  t.bad = !(r.s1 == r.s1) || r.m == INFINITY;
+  t.empty = !t.bad && r.m == -INFINITY;
+  const float nan = __int_as_float(0x7fffffff);
+  t.m = t.bad ? nan : r.m;
+  t.s = t.bad ? nan : t.empty ? 0.0f : r.s;
+  t.s1 = t.bad ? nan : t.empty ? 0.0f : r.s1;
+  t.log_s = t.bad ? nan : t.empty ? -INFINITY : (float)log_det((double)r.s);
+  return t;
+}
+
+// order of the top list: larger values first, of equal values the lower
+// index; keys are distinct, 0 is below every key
+DI unsigned long long top_key(float v, uint32_t index) {
+  const uint32_t b = __float_as_uint(fadd(v, 0.0f));  // -0 and +0 are equal
+  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return ((unsigned long long)o << 32) | (0xffffffffu - index);
+}
+DI float key_value(unsigned long long key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+struct Logits {
+  const void* x;
+  const uint32_t* rows;  // null: row i of the call is row i of x
+  unsigned long long ld;
+  int n, vocab;
+};
+struct ScoreOut {
+  float *logprob, *entropy, *stats;
+  int32_t* top_ids;
+  float* top_logprobs;
+  int top;
+  uint32_t* flags;
+};
+struct Teacher {
+  const void* ids;
+  const void* u;
+  unsigned long long ld;
+  int id_bytes, dtype, k;
+};
+
+// ---- the teacher's list of one row ---------------------------------------------
+struct ListShared {
+  float red[2][kThreads / 32];
+  int bad[kThreads / 32], some[kThreads / 32];
+};
+struct ListEntry {
+  int id;       // -1: not a valid entry
+  float q;      // its share of the teacher's distribution
+  double logq;
+};
+// thread i < k of the block gets entry i (kThreads >= DET_MAX_TOP); *some: the
+// list has a valid entry; *bad: an id or value that is not allowed
+DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float temp, float one, ListShared& sh, bool* some,
+                           bool* bad) {
+  const int t = threadIdx.x, w = t >> 5, l = t & 31;
+  long long id = -1;
+  float u = -INFINITY;
+  if (t < te.k) {
+    id = load_id(te.ids, te.id_bytes, (size_t)row * te.ld + t);
+    if (id >= 0) u = load_any(te.u, te.dtype, (size_t)row * te.ld + t);
+  }
+  const bool wrong = id >= vocab || (id >= 0 && !(u < INFINITY));  // NaN, +inf or no such token
+  const bool valid = id >= 0 && !wrong && u > -INFINITY;
+  float m = warp_max(valid ? u : -INFINITY);
+  const int anyw = __any_sync(kFull, wrong), anyv = __any_sync(kFull, valid);
+  if (l == 0) {
+    sh.red[0][w] = m;
+    sh.bad[w] = anyw;
+    sh.some[w] = anyv;
+  }
+  __syncthreads();
+  m = -INFINITY;
+  int b = 0, so = 0;
+  for (int i = 0; i < kThreads / 32; i++) {
+    m = fmaxf(m, sh.red[0][i]);
+    b |= sh.bad[i];
+    so |= sh.some[i];
+  }
+  const double du = valid ? ddiv(dsub((double)u, (double)m), (double)temp) : 0.0;
+  const float e = valid ? exp1(fmaxf((float)du, kExpLow), one) : 0.0f;
+  const float ws = warp_sum(e);
+  if (l == 0) sh.red[1][w] = ws;
+  __syncthreads();
+  float s = 0.0f;
+  for (int i = 0; i < kThreads / 32; i++) s = fadd(s, sh.red[1][i]);
+  *some = so != 0;
+  *bad = b != 0;
+  ListEntry r;
+  r.id = valid ? (int)id : -1;
+  r.q = valid ? fdiv(e, s) : 0.0f;
+  r.logq = valid ? dsub(du, log_det((double)s)) : 0.0;
+  return r;
+}
+
+// ---- forward ---------------------------------------------------------------------
+// One block per row, warps take segments in turn.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    forward_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, float* loss, ScoreOut o,
+                   float one) {
+  __shared__ float sm[kMaxSegs], ss[kMaxSegs], sw[kMaxSegs];
+  __shared__ RowStats rs;
+  __shared__ ListShared lsh;
+  __shared__ double dred[kThreads / 32];
+  __shared__ unsigned long long kred[kThreads / 32];
+  const int row = blockIdx.x, V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
+  const int nseg = (V + kSeg - 1) / kSeg;
+  const float inv_t = fdiv(1.0f, temp);
+  for (int g = w; g < nseg; g += kThreads / 32) {
+    float v[kPerLane];
+    constexpr int VEC = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kPerLane / VEC; i++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        const int at = g * kSeg + seg_entry<T>(l, i, j);
+        v[i * VEC + j] = at < V ? to_f32(x[at]) : -INFINITY;
+      }
+    const Sums r = segment_sums(v, inv_t, one);
+    if (l == 0) {
+      sm[g] = r.m;
+      ss[g] = r.s;
+      sw[g] = r.s1;
+    }
+  }
+  __syncthreads();
+  if (w == 0) {
+    const RowStats r = finish_row(join_segments(sm, ss, sw, nseg, inv_t, one));
+    if (l == 0) {
+      rs = r;
+      if (o.stats) {
+        float* st = o.stats + (size_t)row * 4;
+        st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = r.log_s;
+      }
+      if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+    }
+  }
+  __syncthreads();
+  const RowStats r = rs;
+  const float nan = __int_as_float(0x7fffffff);
+  const double log_s = r.empty || r.bad ? 0.0 : log_det((double)r.s);
+  if (loss) {
+    bool some, bad;
+    const ListEntry e = teacher_entry(te, row, V, temp, one, lsh, &some, &bad);
+    double term = 0.0;
+    if (e.id >= 0 && e.q > 0.0f) {
+      const double z = (double)to_f32(x[e.id]);
+      const double logp = r.empty ? (double)-INFINITY : dsub(ddiv(dsub(z, (double)r.m), (double)temp), log_s);
+      term = dmul((double)e.q, dsub(e.logq, logp));
+    }
+    term = warp_sum_d(term);
+    if (l == 0) dred[w] = term;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double s = 0.0;
+      for (int i = 0; i < kThreads / 32; i++) s = dadd(s, dred[i]);
+      loss[row] = bad ? nan : !some ? 0.0f : r.bad ? nan : (float)s;
+      if (bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    if (o.entropy) o.entropy[row] = r.bad ? nan : r.empty ? 0.0f : (float)dsub(log_s, ddiv((double)r.s1, (double)r.s));
+    if (o.logprob) {
+      const long long t = load_id(tokens, id_bytes, row);
+      float v;
+      if (r.bad || t >= V) v = nan;
+      else if (t < 0) v = 0.0f;
+      else if (r.empty) v = -INFINITY;
+      else v = (float)dsub(dsub((double)to_f32(x[t]), (double)r.m), log_s);
+      o.logprob[row] = v;
+      if (t >= V && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
+    }
+  }
+  unsigned long long last = ~0ull;
+  for (int k = 0; k < o.top; k++) {
+    unsigned long long best = 0;
+    for (int i = threadIdx.x; i < V; i += kThreads) {
+      const unsigned long long key = top_key(to_f32(x[i]), (uint32_t)i);
+      if (key < last && key > best) best = key;
+    }
+    for (int s = 16; s > 0; s >>= 1) best = max(best, __shfl_xor_sync(kFull, best, s));
+    __syncthreads();
+    if (l == 0) kred[w] = best;
+    __syncthreads();
+    best = 0;
+    for (int i = 0; i < kThreads / 32; i++) best = max(best, kred[i]);
+    last = best;
+    if (threadIdx.x == 0) {
+      const size_t at = (size_t)row * o.top + k;
+      if (o.top_ids) o.top_ids[at] = r.bad ? -1 : (int32_t)(0xffffffffu - (uint32_t)best);
+      if (o.top_logprobs) {
+        o.top_logprobs[at] = r.bad     ? nan
+                             : r.empty ? -INFINITY
+                                       : (float)dsub(dsub((double)key_value(best), (double)r.m), log_s);
+      }
+    }
+  }
+}
+
+// ---- gradient ----------------------------------------------------------------------
+// dx_j = exp(d_j) (a + b d_j) + (what the row's own tokens add): one block per
+// row.  `out` may be the logits themselves.
+struct GradIn {
+  const float *stats, *g, *gh;  // g: of logprob or of the loss; gh: of the entropy, or null
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    grad_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, T* out,
+                unsigned long long out_ld, float one_) {
+  __shared__ ListShared lsh;
+  __shared__ int ids[DET_MAX_TOP];
+  __shared__ float add[DET_MAX_TOP];
+  const int row = blockIdx.x, V = L.vocab;
+  const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
+  T* y = out + (size_t)row * out_ld;
+  const float *st = in.stats + (size_t)row * 4, nan = __int_as_float(0x7fffffff);
+  const float inv_t = fdiv(1.0f, temp);
+  const float m = st[0], s = st[1], s1 = st[2];
+  const bool empty = m == -INFINITY;
+  const float g = in.g ? in.g[row] : 0.0f;
+  float a, b = 0.0f;
+  int k = 0;
+  if (te.k) {
+    bool some, bad;
+    const ListEntry e = teacher_entry(te, row, V, temp, one_, lsh, &some, &bad);
+    const float gt = fdiv(g, temp);
+    a = bad ? nan : !some || empty ? 0.0f : gt;
+    if (!some && !bad) b = nan;  // marks a row without a list: zeros whatever its logits
+    if (threadIdx.x < te.k) {
+      ids[threadIdx.x] = e.id;
+      add[threadIdx.x] = e.q;
+    }
+    __syncthreads();
+    // an id that is listed twice: its first entry takes the sum, in order
+    float sum = 0.0f;
+    if (threadIdx.x < te.k && e.id >= 0) {
+      bool first = true;
+      for (int i = 0; i < te.k; i++)
+        if (ids[i] == e.id) {
+          if (i < (int)threadIdx.x) first = false;
+          sum = fadd(sum, add[i]);
+        }
+      if (!first) sum = -1.0f;
+    }
+    __syncthreads();
+    if (threadIdx.x < te.k) {
+      if (sum < 0.0f) ids[threadIdx.x] = -1;
+      add[threadIdx.x] = fmul(-a, sum);
+    }
+    k = te.k;
+  } else {
+    const float gh = in.gh ? in.gh[row] : 0.0f;
+    const long long t = in.g ? load_id(tokens, id_bytes, row) : -1;
+    const float gl = t < 0 ? 0.0f : t >= V ? nan : g;
+    a = empty ? 0.0f : fadd(-gl, fmul(gh, fdiv(s1, s)));
+    b = empty ? 0.0f : -gh;
+    if (threadIdx.x == 0) {
+      ids[0] = t >= 0 && t < V ? (int)t : -1;
+      add[0] = empty ? 0.0f : gl;
+    }
+    k = 1;
+  }
+  const bool blank = te.k && !(b == b);
+  if (blank) b = 0.0f;
+  __syncthreads();
+  const float base = empty ? 0.0f : -m, inv_s = empty ? 0.0f : fdiv(1.0f, s);
+  const float as = fmul(a, inv_s), bs = fmul(b, inv_s);
+  const f2 one = pk(one_, one_);
+  auto grad = [&](float v) {
+    const Exp2 e = exp2_lanes(mul2(add2(pk(v, v), pk(base, base)), pk(inv_t, inv_t)), one);
+    const f2 c = b == 0.0f ? pk(as, as) : addp(mul2(e.d, pk(bs, bs)), one, pk(as, as));
+    const float r = un(mul2(e.e, c)).x;
+    return blank || empty ? 0.0f : r;
+  };
+  // the values at the row's own tokens, before `out` may overwrite them
+  float mine = 0.0f;
+  const int id = threadIdx.x < k ? ids[threadIdx.x] : -1;
+  if (id >= 0) mine = fadd(grad(to_f32(x[id])), add[threadIdx.x]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < V; i += kThreads) y[i] = from_f32<T>(grad(to_f32(x[i])));
+  __syncthreads();
+  if (id >= 0 && !blank && !empty) y[id] = from_f32<T>(mine);
+}
+
+// ---- launches --------------------------------------------------------------------
+template <typename F>
+cudaError_t by_dtype(int dtype, F f) {
+  switch (dtype) {
+    case DET_DTYPE_F32: f(float{}); break;
+    case DET_DTYPE_F16: f(__half{}); break;
+    default: f(__nv_bfloat16{}); break;
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_forward(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
+                           const Teacher& te, float temp, float* loss, const ScoreOut& o) {
+  return by_dtype(dtype, [&](auto t) {
+    forward_kernel<decltype(t)><<<L.n, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, loss, o, 1.0f);
+  });
+}
+cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
+                        const Teacher& te, float temp, const GradIn& in, void* out, unsigned long long out_ld) {
+  return by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    grad_kernel<T><<<L.n, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, static_cast<T*>(out), out_ld, 1.0f);
+  });
+}
+
+// ---- argument checks ----------------------------------------------------------------
+size_t dtype_size(int dtype) { return dtype == DET_DTYPE_F32 ? 4 : 2; }
+
+det_status check_logits(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld) {
+  if (!logits || dtype < DET_DTYPE_F32 || dtype > DET_DTYPE_BF16) return DET_ERR_INVALID_ARGUMENT;
+  if (vocab == 0) return DET_ERR_CDF_EMPTY;
+  if (vocab > kMaxVocab) return DET_ERR_CDF_TOO_MANY_SYMBOLS;
+  if (n > DET_SCORE_MAX_ROWS || ld > (1ull << 40)) return DET_ERR_INVALID_ARGUMENT;
+  if ((uintptr_t)logits % dtype_size(dtype)) return DET_ERR_INVALID_ARGUMENT;
+  return DET_OK;
+}
+// the gradient goes over the logits exactly, or nowhere near them: equal
+// strides side by side, or ranges that do not meet
+det_status check_grad(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld, const void* grad,
+                      uint64_t grad_ld) {
+  if (!grad || (n > 1 && grad_ld < vocab) || grad_ld > (1ull << 40)) return DET_ERR_INVALID_ARGUMENT;
+  const size_t sz = dtype_size(dtype);
+  if ((uintptr_t)grad % sz) return DET_ERR_INVALID_ARGUMENT;
+  const uintptr_t a = (uintptr_t)logits, b = (uintptr_t)grad;
+  if (a == b) return n == 1 || ld == grad_ld ? DET_OK : DET_ERR_INVALID_ARGUMENT;
+  const size_t an = ((size_t)(n - 1) * ld + vocab) * sz, bn = ((size_t)(n - 1) * grad_ld + vocab) * sz;
+  if (a + an <= b || b + bn <= a) return DET_OK;
+  if (n == 1 || ld != grad_ld) return DET_ERR_INVALID_ARGUMENT;
+  const size_t pitch = ld * sz, off = (b > a ? b - a : pitch - (a - b) % pitch) % pitch, row = vocab * sz;
+  return off >= row && off + row <= pitch ? DET_OK : DET_ERR_INVALID_ARGUMENT;
+}
+det_status check_ids(const void* ids, int id_bytes) {
+  if (!ids || (id_bytes != 4 && id_bytes != 8) || (uintptr_t)ids % id_bytes) return DET_ERR_INVALID_ARGUMENT;
+  return DET_OK;
+}
+det_status check_list(const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k, uint32_t n,
+                      uint64_t ld, float temperature) {
+  if (det_status st = check_ids(ids, id_bytes)) return st;
+  if (!teacher || teacher_dtype < DET_DTYPE_F32 || teacher_dtype > DET_DTYPE_BF16 ||
+      (uintptr_t)teacher % dtype_size(teacher_dtype))
+    return DET_ERR_INVALID_ARGUMENT;
+  if (k == 0 || k > DET_MAX_TOP || (n > 1 && ld < k) || ld > (1ull << 40)) return DET_ERR_INVALID_ARGUMENT;
+  if (!(temperature >= DET_MIN_TEMPERATURE && temperature <= DET_MAX_TEMPERATURE)) return DET_ERR_INVALID_ARGUMENT;
+  return DET_OK;
+}
+det_status check_device() {
+  int cnt = 0;
+  return cudaGetDeviceCount(&cnt) != cudaSuccess || cnt == 0 ? DET_ERR_NO_DEVICE : DET_OK;
+}
+det_status launched(cudaError_t e) {
+  return e == cudaSuccess ? DET_OK : e == cudaErrorMemoryAllocation ? DET_ERR_DEVICE_OOM : DET_ERR_CUDA;
+}
+
+const Teacher kNoTeacher{nullptr, nullptr, 0, 4, DET_DTYPE_F32, 0};
+
+}  // namespace
+
+cudaError_t launch_token_scores(const Launch& L, const float* logits, int V, const uint32_t* rows,
+                                const uint32_t* tokens, int n, int top, float* logprob, float* entropy,
+                                int32_t* top_ids, float* top_logprobs) {
+  const Logits x{logits, rows, (unsigned long long)V, n, V};
+  const ScoreOut o{logprob, entropy, nullptr, top_ids, top_logprobs, top, L.err};
+  if (L.launches) ++*L.launches;
+  return launch_forward(L.stream, DET_DTYPE_F32, x, tokens, 4, kNoTeacher, 1.0f, nullptr, o);
+}
+cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, const uint32_t* rows, int n,
+                                const int32_t* ids, const float* teacher, int k, float temperature, float* loss) {
+  const Logits x{logits, rows, (unsigned long long)V, n, V};
+  const Teacher te{ids, teacher, (unsigned long long)k, 4, DET_DTYPE_F32, k};
+  const ScoreOut o{nullptr, nullptr, nullptr, nullptr, nullptr, 0, L.err};
+  if (L.launches) ++*L.launches;
+  return launch_forward(L.stream, DET_DTYPE_F32, x, nullptr, 4, te, temperature, loss, o);
+}
+
+static_assert(DET_SCORE_NONFINITE == (int)ERRF_CDF_NONFINITE && DET_SCORE_BAD_TOKEN == (int)ERRF_SYMBOL,
+              "the flags are the session's error bits");
+}  // namespace det
+
+using namespace det;
+
+extern "C" {
+
+det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* tokens, int token_bytes, uint32_t top, float* logprob, float* entropy,
+                                   float* stats, int32_t* top_ids, float* top_logprobs, uint32_t* flags,
+                                   void* stream) {
+  if (n == 0) return DET_OK;
+  if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
+  if (logprob)
+    if (det_status st = check_ids(tokens, token_bytes)) return st;
+  if (top > DET_MAX_TOP || top > vocab || (top && !top_ids && !top_logprobs)) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_device()) return st;
+  const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
+  const ScoreOut o{logprob, entropy, stats, top_ids, top_logprobs, (int)top, flags};
+  return launched(launch_forward(static_cast<cudaStream_t>(stream), dtype, L, tokens, token_bytes, kNoTeacher, 1.0f,
+                                 nullptr, o));
+}
+
+det_status det_token_scores_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                        const void* tokens, int token_bytes, const float* stats,
+                                        const float* grad_logprob, const float* grad_entropy, void* grad,
+                                        uint64_t grad_ld, void* stream) {
+  if (n == 0) return DET_OK;
+  if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
+  if (det_status st = check_grad(logits, dtype, n, vocab, ld, grad, grad_ld)) return st;
+  if (!stats || (!grad_logprob && !grad_entropy)) return DET_ERR_INVALID_ARGUMENT;
+  if (grad_logprob)
+    if (det_status st = check_ids(tokens, token_bytes)) return st;
+  if (det_status st = check_device()) return st;
+  const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
+  return launched(launch_grad(static_cast<cudaStream_t>(stream), dtype, L, tokens, token_bytes, kNoTeacher, 1.0f,
+                              GradIn{stats, grad_logprob, grad_entropy}, grad, grad_ld));
+}
+
+det_status det_token_scores_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                        const void* tokens, int token_bytes, const float* grad_logprob,
+                                        const float* grad_entropy, float* logprob, float* entropy, float* stats,
+                                        void* grad, uint64_t grad_ld, uint32_t* flags, void* stream) {
+  if (n == 0) return DET_OK;
+  if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
+  if (det_status st = check_grad(logits, dtype, n, vocab, ld, grad, grad_ld)) return st;
+  if (!stats || (!grad_logprob && !grad_entropy)) return DET_ERR_INVALID_ARGUMENT;
+  if (logprob || grad_logprob)
+    if (det_status st = check_ids(tokens, token_bytes)) return st;
+  if (det_status st = check_device()) return st;
+  const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
+  const ScoreOut o{logprob, entropy, stats, nullptr, nullptr, 0, flags};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cudaError_t e = launch_forward(s, dtype, L, tokens, token_bytes, kNoTeacher, 1.0f, nullptr, o))
+    return launched(e);
+  return launched(launch_grad(s, dtype, L, tokens, token_bytes, kNoTeacher, 1.0f,
+                              GradIn{stats, grad_logprob, grad_entropy}, grad, grad_ld));
+}
+
+det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
+                                   uint64_t list_ld, float temperature, float* loss, float* stats, uint32_t* flags,
+                                   void* stream) {
+  if (n == 0) return DET_OK;
+  if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
+  if (det_status st = check_list(ids, id_bytes, teacher, teacher_dtype, k, n, list_ld, temperature)) return st;
+  if (!loss) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_device()) return st;
+  const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
+  const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
+  const ScoreOut o{nullptr, nullptr, stats, nullptr, nullptr, 0, flags};
+  return launched(launch_forward(static_cast<cudaStream_t>(stream), dtype, L, nullptr, 4, te, temperature, loss, o));
+}
+
+det_status det_distill_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
+                                   uint64_t list_ld, float temperature, const float* stats, const float* grad_loss,
+                                   void* grad, uint64_t grad_ld, void* stream) {
+  if (n == 0) return DET_OK;
+  if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
+  if (det_status st = check_grad(logits, dtype, n, vocab, ld, grad, grad_ld)) return st;
+  if (det_status st = check_list(ids, id_bytes, teacher, teacher_dtype, k, n, list_ld, temperature)) return st;
+  if (!stats || !grad_loss) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_device()) return st;
+  const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
+  const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
+  return launched(launch_grad(static_cast<cudaStream_t>(stream), dtype, L, nullptr, 4, te, temperature,
+                              GradIn{stats, grad_loss, nullptr}, grad, grad_ld));
+}
+
+det_status det_distill_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
+                                   uint64_t list_ld, float temperature, const float* grad_loss, float* loss,
+                                   float* stats, void* grad, uint64_t grad_ld, uint32_t* flags, void* stream) {
+  if (n == 0) return DET_OK;
+  if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
+  if (det_status st = check_grad(logits, dtype, n, vocab, ld, grad, grad_ld)) return st;
+  if (det_status st = check_list(ids, id_bytes, teacher, teacher_dtype, k, n, list_ld, temperature)) return st;
+  if (!loss || !stats || !grad_loss) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_device()) return st;
+  const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
+  const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
+  const ScoreOut o{nullptr, nullptr, stats, nullptr, nullptr, 0, flags};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cudaError_t e = launch_forward(s, dtype, L, nullptr, 4, te, temperature, loss, o)) return launched(e);
+  return launched(
+      launch_grad(s, dtype, L, nullptr, 4, te, temperature, GradIn{stats, grad_loss, nullptr}, grad, grad_ld));
+}
+
+}  // extern "C"

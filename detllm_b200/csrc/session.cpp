@@ -7,6 +7,7 @@
 // for all n positions before the next op, which leaves each position's
 // arithmetic unchanged (each reduction stays within one position).
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 
@@ -123,7 +124,7 @@ void free_session(det_session* s) {
   for (void* p : s->allocations) cudaFree(p);
   if (s->graph_dev1.exec) cudaGraphExecDestroy(s->graph_dev1.exec);
   for (void* p : {(void*)s->h_tokens, (void*)s->h_rows, (void*)s->h_syms, (void*)s->h_err, (void*)s->h_out,
-                  (void*)s->h_value, (void*)s->h_pos, (void*)s->h_rc})
+                  (void*)s->h_value, (void*)s->h_pos, (void*)s->h_rc, (void*)s->h_score})
     if (p) cudaFreeHost(p);
   for (auto& e : s->ev)
     if (e) cudaEventDestroy(e);
@@ -964,6 +965,120 @@ det_status det_decoder_lookup(det_session* s, uint32_t row, int byte_escapes, ui
   out->freq = (uint32_t)s->h_out[2];
   out->reserved = 0;
   out->total = s->h_out[3];
+  return DET_OK;
+}
+
+// ---- token scores and distillation (scoring.cu) --------------------------
+// d_score / h_score hold one group of up to 1,024 rows: 16 bytes per row
+// (token or loss, logprob, entropy) and 8 per list entry (id, value).
+static constexpr uint32_t kScoreRows = 1024;
+static det_status score_buffers(det_session* s) {
+  const size_t bytes = (size_t)kScoreRows * (16 + 8 * DET_MAX_TOP);
+  if (!s->d_score)
+    if (det_status st = dalloc(s, &s->d_score, bytes)) return st;
+  return s->h_score ? DET_OK : halloc(s, &s->h_score, bytes);
+}
+
+// a group's rows, checked, into h_rows (copied to the device by the caller)
+static det_status score_rows(det_session* s, const uint32_t* rows, uint32_t base, uint32_t cnt) {
+  for (uint32_t i = 0; i < cnt; i++) {
+    s->h_rows[i] = rows ? rows[base + i] : base + i;
+    if (s->h_rows[i] >= (uint32_t)s->last_n) return DET_ERR_SHAPE;
+  }
+  return DET_OK;
+}
+
+det_status det_token_scores(det_session* s, const uint32_t* rows, const uint32_t* tokens, uint32_t n, uint32_t top,
+                            float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs) {
+  if (!s || (n && (!tokens || !logprob || !entropy))) return DET_ERR_INVALID_ARGUMENT;
+  if (top > DET_MAX_TOP || (n && top && (!top_ids || !top_logprobs))) return DET_ERR_INVALID_ARGUMENT;
+  if (n == 0) return DET_OK;
+  if (top > (uint32_t)s->m->vocab) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_symbols(s, 0)) return st;
+  const uint32_t V = (uint32_t)s->m->vocab;
+  cudaSetDevice(s->m->device);
+  if (det_status st = score_buffers(s)) return st;
+  for (uint32_t base = 0; base < n; base += kScoreRows) {
+    const uint32_t cnt = std::min(kScoreRows, n - base);
+    if (det_status st = score_rows(s, rows, base, cnt)) return st;
+    // tokens | logprob | entropy | top logprobs | top ids
+    uint32_t* ht = reinterpret_cast<uint32_t*>(s->h_score);
+    for (uint32_t i = 0; i < cnt; i++) {
+      ht[i] = tokens[base + i];
+      if (ht[i] >= V && ht[i] != UINT32_MAX) return DET_ERR_CDF_SYMBOL_OUT_OF_RANGE;
+    }
+    CK(cudaEventRecord(s->ev[2], s->stream));
+    CK(cudaMemcpyAsync(s->d_rows + 1024, s->h_rows, cnt * 4, cudaMemcpyHostToDevice, s->stream));
+    CK(cudaMemcpyAsync(s->d_score, s->h_score, cnt * 4, cudaMemcpyHostToDevice, s->stream));
+    s->stats.h2d_bytes += cnt * 8;
+    float* d = reinterpret_cast<float*>(s->d_score) + cnt;
+    const size_t list = (size_t)cnt * top;
+    CK(timed(s, PT_CDF, 0, 0, [&] {
+      return launch_token_scores(launch_of(s), s->logits, (int)V, s->d_rows + 1024,
+                                 reinterpret_cast<const uint32_t*>(s->d_score), (int)cnt, (int)top, d, d + cnt,
+                                 reinterpret_cast<int32_t*>(d + 2 * cnt + list), d + 2 * cnt);
+    }));
+    CK(cudaEventRecord(s->ev[3], s->stream));
+    const size_t words = 2 * (size_t)cnt + 2 * list;
+    CK(cudaMemcpyAsync(s->h_score, d, words * 4, cudaMemcpyDeviceToHost, s->stream));
+    s->stats.d2h_bytes += words * 4;
+    if (det_status st = take_error(s, true)) return st;
+    forward_collect(s);
+    float ms = 0.0f;
+    if (cudaEventElapsedTime(&ms, s->ev[2], s->ev[3]) == cudaSuccess) s->stats.cdf_ms += ms;
+    const float* h = reinterpret_cast<const float*>(s->h_score);
+    std::memcpy(logprob + base, h, cnt * 4);
+    std::memcpy(entropy + base, h + cnt, cnt * 4);
+    if (top) {
+      std::memcpy(top_logprobs + (size_t)base * top, h + 2 * cnt, list * 4);
+      std::memcpy(top_ids + (size_t)base * top, h + 2 * cnt + list, list * 4);
+    }
+  }
+  return DET_OK;
+}
+
+det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, const uint32_t* teacher_ids,
+                            const float* teacher_logits, uint32_t k, float temperature, float* loss) {
+  if (!s || (n && (!teacher_ids || !teacher_logits || !loss))) return DET_ERR_INVALID_ARGUMENT;
+  if (k == 0 || k > DET_MAX_TOP) return DET_ERR_INVALID_ARGUMENT;
+  if (!(temperature >= DET_MIN_TEMPERATURE && temperature <= DET_MAX_TEMPERATURE)) return DET_ERR_INVALID_ARGUMENT;
+  if (n == 0) return DET_OK;
+  if (det_status st = check_symbols(s, 0)) return st;
+  const uint32_t V = (uint32_t)s->m->vocab;
+  cudaSetDevice(s->m->device);
+  if (det_status st = score_buffers(s)) return st;
+  for (uint32_t base = 0; base < n; base += kScoreRows) {
+    const uint32_t cnt = std::min(kScoreRows, n - base);
+    if (det_status st = score_rows(s, rows, base, cnt)) return st;
+    // ids | values | loss
+    const size_t list = (size_t)cnt * k;
+    uint32_t* hi = reinterpret_cast<uint32_t*>(s->h_score);
+    float* hu = reinterpret_cast<float*>(s->h_score) + list;
+    for (size_t i = 0; i < list; i++) {
+      hi[i] = teacher_ids[(size_t)base * k + i];
+      hu[i] = teacher_logits[(size_t)base * k + i];
+      if (hi[i] == UINT32_MAX) continue;  // no entry
+      if (hi[i] >= V) return DET_ERR_CDF_SYMBOL_OUT_OF_RANGE;
+      if (!(hu[i] < INFINITY)) return DET_ERR_CDF_NONFINITE_LOGIT;
+    }
+    CK(cudaEventRecord(s->ev[2], s->stream));
+    CK(cudaMemcpyAsync(s->d_rows + 1024, s->h_rows, cnt * 4, cudaMemcpyHostToDevice, s->stream));
+    CK(cudaMemcpyAsync(s->d_score, s->h_score, list * 8, cudaMemcpyHostToDevice, s->stream));
+    s->stats.h2d_bytes += cnt * 4 + list * 8;
+    float* d = reinterpret_cast<float*>(s->d_score);
+    CK(timed(s, PT_CDF, 0, 0, [&] {
+      return launch_distill_loss(launch_of(s), s->logits, (int)V, s->d_rows + 1024, (int)cnt,
+                                 reinterpret_cast<const int32_t*>(d), d + list, (int)k, temperature, d + 2 * list);
+    }));
+    CK(cudaEventRecord(s->ev[3], s->stream));
+    CK(cudaMemcpyAsync(s->h_score, d + 2 * list, cnt * 4, cudaMemcpyDeviceToHost, s->stream));
+    s->stats.d2h_bytes += cnt * 4;
+    if (det_status st = take_error(s, true)) return st;
+    forward_collect(s);
+    float ms = 0.0f;
+    if (cudaEventElapsedTime(&ms, s->ev[2], s->ev[3]) == cudaSuccess) s->stats.cdf_ms += ms;
+    std::memcpy(loss + base, s->h_score, cnt * 4);
+  }
   return DET_OK;
 }
 

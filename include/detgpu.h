@@ -306,6 +306,94 @@ det_status det_model_profile(det_model* model, char* out, size_t cap, int reset)
 det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t vocab, const uint32_t* symbols,
                                      int byte_escapes, det_symbol_range* out, void* stream);
 
+/* ---- token scores and distillation (no counterpart in the reference) ------
+ * What the logits say about tokens.  For a row x of `vocab` logits, with
+ * m = max x, d_j = (x_j - m) / T, S = sum exp(d_j), S1 = sum exp(d_j) d_j:
+ *
+ *   log p_j = d_j - log S          natural logarithms; -log2 p is the length
+ *   entropy = log S - S1 / S       of the token's ideal code, in bits
+ *   loss    = sum_i q_i (log q_i - log p_id(i)),  q = softmax(u / T) over the
+ *             valid entries of a teacher's list (id, u); T = 1 for scores
+ *
+ * An entry of -inf is masked out: its probability is 0.  What a row gives:
+ *   token < 0                  ignored: logprob 0, no gradient through it
+ *   token or id >= vocab       NaN, and DET_SCORE_BAD_TOKEN in *flags
+ *   NaN or +inf in the row     NaN and top ids -1, DET_SCORE_NONFINITE
+ *   nothing but -inf           logprob -inf, entropy 0, loss +inf, gradient 0
+ *   list entry: id < 0, u -inf not a valid entry; u NaN or +inf: as a bad id
+ *   no valid entry in a list   loss 0 and gradient 0, whatever the logits
+ *   an id listed twice         two terms of the loss; its gradient has both
+ * A probability below exp(-88) of the row's largest counts as 0.
+ *
+ * Results are deterministic, and a row's are the same bits in whatever batch,
+ * stride or call it is (the sums' order depends on the vocabulary and the
+ * element type alone).  They are not specified bit for bit across library
+ * versions.
+ *
+ * The *_device calls work on the caller's device memory, on `stream` of the
+ * calling thread's current device.  They allocate nothing, keep nothing and
+ * do not synchronise, so they can be captured into a graph and may overlap
+ * each other.  Pointers are aligned to their element.  Row i of the logits
+ * starts ld elements after row i - 1; lists likewise (list_ld); what lies
+ * between rows is neither read nor written.  dtype: DET_DTYPE_*.  token_bytes
+ * / id_bytes: 4 (int32) or 8 (int64).  *flags (or NULL) gets bits OR-ed in
+ * and is never cleared.  `stats` holds 4 floats per row, m, S, S1, log S: the
+ * gradient calls read what the forward calls wrote for the same logits.
+ * Output pointers may be NULL where not needed, except `loss`, `grad` and, in
+ * the gradient and step calls, `stats`.
+ *
+ * `grad` has the logits' type and gets one rounding.  It may be the logits
+ * themselves (same pointer and stride), or side by side with them in rows of
+ * one stride; any other overlap is DET_ERR_INVALID_ARGUMENT. */
+enum { DET_DTYPE_F32 = 0, DET_DTYPE_F16 = 1, DET_DTYPE_BF16 = 2 };
+enum { DET_SCORE_NONFINITE = 2, DET_SCORE_BAD_TOKEN = 64 };
+#define DET_MAX_TOP 128u
+#define DET_SCORE_MAX_ROWS (1u << 26)
+#define DET_MIN_TEMPERATURE 1e-6f
+#define DET_MAX_TEMPERATURE 1e6f
+/* On a session, beside det_symbol_ranges: output i is about row rows[i] of
+ * the last det_forward (rows == NULL: row i), with host arrays.  tokens[i] ==
+ * UINT32_MAX is ignored and so is a list entry with that id; a token or id
+ * outside the vocabulary is DET_ERR_CDF_SYMBOL_OUT_OF_RANGE, a logit that is
+ * not finite DET_ERR_CDF_NONFINITE_LOGIT. */
+det_status det_token_scores(det_session* s, const uint32_t* rows, const uint32_t* tokens, uint32_t n, uint32_t top,
+                            float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs);
+det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, const uint32_t* teacher_ids,
+                            const float* teacher_logits, uint32_t k, float temperature, float* loss);
+/* log probability of tokens[i], entropy, and the `top` (<= DET_MAX_TOP, <=
+ * vocab) most likely tokens of row i with their log probabilities, most
+ * likely first, equal ones in the order of their ids: n x top each */
+det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* tokens, int token_bytes, uint32_t top, float* logprob, float* entropy,
+                                   float* stats, int32_t* top_ids, float* top_logprobs, uint32_t* flags, void* stream);
+/* grad = d (sum_i grad_logprob[i] logprob[i] + grad_entropy[i] entropy[i]) /
+ * d logits; either of the two may be NULL */
+det_status det_token_scores_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                        const void* tokens, int token_bytes, const float* stats,
+                                        const float* grad_logprob, const float* grad_entropy, void* grad,
+                                        uint64_t grad_ld, void* stream);
+/* both in one call: the logits are read once */
+det_status det_token_scores_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                        const void* tokens, int token_bytes, const float* grad_logprob,
+                                        const float* grad_entropy, float* logprob, float* entropy, float* stats,
+                                        void* grad, uint64_t grad_ld, uint32_t* flags, void* stream);
+/* loss[i] of row i against the k (1 .. DET_MAX_TOP) entries of list i, at
+ * temperature T (DET_MIN_TEMPERATURE .. DET_MAX_TEMPERATURE) on both sides */
+det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
+                                   uint64_t list_ld, float temperature, float* loss, float* stats, uint32_t* flags,
+                                   void* stream);
+/* grad = d (sum_i grad_loss[i] loss[i]) / d logits (the teacher has none) */
+det_status det_distill_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
+                                   uint64_t list_ld, float temperature, const float* stats, const float* grad_loss,
+                                   void* grad, uint64_t grad_ld, void* stream);
+/* both in one call: the logits are read once */
+det_status det_distill_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
+                                   const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
+                                   uint64_t list_ld, float temperature, const float* grad_loss, float* loss,
+                                   float* stats, void* grad, uint64_t grad_ld, uint32_t* flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
