@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cstring>
 #include <type_traits>
 
 #include "../../include/detgpu.h"
@@ -132,11 +133,90 @@ DI long long load_id(const void* p, int bytes, size_t i) {
 }
 
 // ---- a segment -------------------------------------------------------------------
-// entry of lane l, vector i, element j of a segment
+// Lane l's vector i of a segment holds its entries (32 i + l) VEC + j.
 template <typename T>
-DI int seg_entry(int l, int i, int j) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  return i * 32 * VEC + l * VEC + j;
+struct Seg {
+  static constexpr int VEC = 16 / (int)sizeof(T);     // entries per 16 bytes
+  static constexpr int NV = kPerLane / VEC;           // vectors per lane
+  static constexpr int GROUP = 32 * VEC;              // adjacent entries a warp loads at once
+};
+
+template <typename T>
+DI void unpack_vec(uint4 w, float* v) {
+  if constexpr (std::is_same_v<T, float>) {
+    v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y);
+    v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
+  } else {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      } else {
+        __half2 h;
+        memcpy(&h, &u[i], 4);
+        const float2 f = __half22float2(h);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+// 16 bytes that start `bytes` (< 16, even) into the 32 of a and b; `bytes` is
+// the same in every lane
+DI uint4 shifted(uint4 a, uint4 b, int bytes) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (bytes & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+  }
+  if (bytes & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = w[i + 1];
+  }
+  if (bytes & 2) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// VEC entries from entry `at` of a row; what is past its end is -inf.  Only
+// 16-byte granules that lie in the row as a whole are loaded as such: a row
+// that starts `mis` entries into a granule takes two of them per vector.
+template <typename T>
+DI void load_vec(const T* __restrict__ row, int at, int V, int mis, float* v) {
+  constexpr int VEC = Seg<T>::VEC;
+  const T* p = row + at;
+  if (mis == 0 && at + VEC <= V) {
+    unpack_vec<T>(__ldg(reinterpret_cast<const uint4*>(p)), v);
+  } else if (mis != 0 && at >= mis && at - mis + 2 * VEC <= V) {
+    const uint4* q = reinterpret_cast<const uint4*>(p - mis);
+    unpack_vec<T>(shifted(__ldg(q), __ldg(q + 1), mis * (int)sizeof(T)), v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) v[j] = at + j < V ? to_f32(p[j]) : -INFINITY;
+  }
+}
+template <typename T>
+DI int misaligned(const T* row) {
+  return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+template <typename T>
+DI void load_segment(const T* __restrict__ row, int g, int V, int mis, float (&v)[kPerLane]) {
+  using G = Seg<T>;
+  const int base = g * kSeg + (threadIdx.x & 31) * G::VEC;
+  if (mis == 0 && (g + 1) * kSeg <= V) {
+    const uint4* p = reinterpret_cast<const uint4*>(row + base);
+    uint4 w[G::NV];
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) w[i] = __ldg(p + 32 * i);
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) unpack_vec<T>(w[i], v + i * G::VEC);
+  } else {
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) load_vec<T>(row, base + i * G::GROUP, V, mis, v + i * G::VEC);
+  }
 }
 
 struct Sums {
@@ -157,23 +237,28 @@ DI double warp_sum_d(double v) {
 }
 
 // maximum, sum of exp((x - m) / T) and the same weighted by (x - m) / T over
-// one segment's 64 entries per lane; a NaN or +inf anywhere leaves s1 NaN
-DI Sums segment_sums(const float (&x)[kPerLane], float inv_t, float one_) {
-  float m = x[0];
-#pragma unroll
-  for (int i = 1; i < kPerLane; i++) m = fmaxf(m, x[i]);
-  m = warp_max(m);
+// one segment's 64 entries per lane; a NaN or +inf anywhere leaves s1 NaN.
+// `m`: the segment's maximum.
+template <bool SCALED>
+DI Sums segment_sums(const float (&x)[kPerLane], float m, float inv_t, float one_) {
   const float base = m == -INFINITY ? 0.0f : -m;
   const f2 nm = pk(base, base), one = pk(one_, one_), it = pk(inv_t, inv_t);
   f2 s[2] = {0, 0}, w[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < kPerLane / 2; i++) {
-    const Exp2 e = exp2_lanes(mul2(add2(pk(x[2 * i], x[2 * i + 1]), nm), it), one);
+    f2 d = add2(pk(x[2 * i], x[2 * i + 1]), nm);
+    if constexpr (SCALED) d = mul2(d, it);
+    const Exp2 e = exp2_lanes(d, one);
     s[i & 1] = add2(s[i & 1], e.e);
     w[i & 1] = addp(mul2(e.e, e.d), one, w[i & 1]);
   }
   const float2 sp = un(add2(s[0], s[1])), wp = un(add2(w[0], w[1]));
   return {m, warp_sum(fadd(sp.x, sp.y)), warp_sum(fadd(wp.x, wp.y))};
+}
+DI float redux_max(float v) {  // of the warp; a NaN loses against a number
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(kFull));
+  return r;
 }
 
 // joins a row's segments (one warp; the result in every lane)
@@ -195,7 +280,8 @@ DI Sums join_segments(const float* sm, const float* ss, const float* sw, int nse
 }
 
 struct RowStats {
-  float m, s, s1, log_s;
+  float m, s, s1;
+  double log_s;
   bool empty, bad;
 };
 DI RowStats finish_row(const Sums& r) {
@@ -206,7 +292,7 @@ DI RowStats finish_row(const Sums& r) {
   t.m = t.bad ? nan : r.m;
   t.s = t.bad ? nan : t.empty ? 0.0f : r.s;
   t.s1 = t.bad ? nan : t.empty ? 0.0f : r.s1;
-  t.log_s = t.bad ? nan : t.empty ? -INFINITY : (float)log_det((double)r.s);
+  t.log_s = t.bad ? (double)nan : t.empty ? (double)-INFINITY : log_det((double)r.s);
   return t;
 }
 
@@ -296,108 +382,311 @@ DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float temp, fl
   return r;
 }
 
-// ---- forward ---------------------------------------------------------------------
-// One block per row, warps take segments in turn.
+// ---- the top list ------------------------------------------------------------------
+// The maximum of every group of adjacent entries is kept while a row's sums
+// are taken; the k largest entries lie in the groups whose maxima are among
+// the k largest, so only those are read again.  A group is what a warp loads
+// at once (128 f32 or 256 16-bit entries), or one lane's 16 bytes of it where
+// that would leave too few groups for a list (vocabularies up to 32,768).
+constexpr int kSmallVocab = 32768;
+constexpr int kCand = 2048;  // keys held before they are cut down to k
+struct TopShared {
+  unsigned long long key[kCand + kThreads];
+  int count, bits[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    forward_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, float* loss, ScoreOut o,
-                   float one) {
-  __shared__ float sm[kMaxSegs], ss[kMaxSegs], sw[kMaxSegs];
-  __shared__ RowStats rs;
-  __shared__ ListShared lsh;
-  __shared__ double dred[kThreads / 32];
-  __shared__ unsigned long long kred[kThreads / 32];
-  const int row = blockIdx.x, V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
-  const int nseg = (V + kSeg - 1) / kSeg;
-  const float inv_t = fdiv(1.0f, temp);
-  for (int g = w; g < nseg; g += kThreads / 32) {
-    float v[kPerLane];
-    constexpr int VEC = 16 / (int)sizeof(T);
+DI int group_size(int V) {
+  return V <= kSmallVocab ? Seg<T>::VEC : Seg<T>::GROUP;
+}
+template <typename T>
+size_t groups_of(int V) {
+  const int g = V <= kSmallVocab ? Seg<T>::VEC : Seg<T>::GROUP, nseg = (V + kSeg - 1) / kSeg;
+  return (size_t)nseg * (kSeg / g);
+}
+
+// the largest t such that at least k of the block's values are >= t (0 where
+// there are fewer than k): bit by bit, done early once exactly k are
+template <typename K, int PER>
+DI K kth_largest(const K (&v)[PER], int k, TopShared& sh) {
+  K t = 0;
+  for (int bit = (int)sizeof(K) * 8 - 1, turn = 0; bit >= 0; bit--, turn ^= 1) {
+    const K cand = t | ((K)1 << bit);
+    int c = 0;
 #pragma unroll
-    for (int i = 0; i < kPerLane / VEC; i++)
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        const int at = g * kSeg + seg_entry<T>(l, i, j);
-        v[i * VEC + j] = at < V ? to_f32(x[at]) : -INFINITY;
-      }
-    const Sums r = segment_sums(v, inv_t, one);
-    if (l == 0) {
-      sm[g] = r.m;
-      ss[g] = r.s;
-      sw[g] = r.s1;
-    }
+    for (int i = 0; i < PER; i++) c += v[i] >= cand;
+    c = __reduce_add_sync(kFull, c);
+    if ((threadIdx.x & 31) == 0 && c) atomicAdd(&sh.bits[turn], c);
+    __syncthreads();
+    const int all = sh.bits[turn];
+    if (threadIdx.x == 0) sh.bits[turn ^ 1] = 0;
+    __syncthreads();
+    if (all >= k) t = cand;
+    if (all == k) break;
   }
   __syncthreads();
-  if (w == 0) {
-    const RowStats r = finish_row(join_segments(sm, ss, sw, nseg, inv_t, one));
+  if (threadIdx.x == 0) sh.bits[0] = sh.bits[1] = 0;
+  __syncthreads();
+  return t;
+}
+// keeps the k largest of the block's sh.count keys (distinct); returns the
+// smallest of them, or 0 if there are fewer than k
+DI unsigned long long cut_to(int k, TopShared& sh) {
+  __syncthreads();
+  const int n = min(sh.count, kCand + kThreads);
+  if (n <= k) {
+    const unsigned long long r = 0;
+    __syncthreads();
+    return r;
+  }
+  constexpr int PER = (kCand + kThreads) / kThreads;
+  unsigned long long v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int at = i * kThreads + threadIdx.x;
+    v[i] = at < n ? sh.key[at] : 0;
+  }
+  const unsigned long long t = kth_largest<unsigned long long, PER>(v, k, sh);
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; i++)
+    if (v[i] >= t) sh.key[atomicAdd(&sh.count, 1)] = v[i];
+  __syncthreads();
+  return t;
+}
+// adds the entries of groups [g0, g1) whose keys are above `floor`
+template <typename T>
+DI void collect(const T* __restrict__ x, int V, int mis, const float* gmax, int g0, int g1, unsigned long long floor,
+                TopShared& sh) {
+  using G = Seg<T>;
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  auto push = [&](float v, int at) {
+    const unsigned long long key = top_key(v, (uint32_t)at);
+    if (at < V && key > floor) {
+      const int slot = atomicAdd(&sh.count, 1);
+      if (slot < kCand + kThreads) sh.key[slot] = key;
+    }
+  };
+  if (V <= kSmallVocab) {
+    for (int g = g0 + threadIdx.x; g < g1; g += kThreads)
+      if (g * G::VEC < V && top_key(gmax[g], (uint32_t)(g * G::VEC)) > floor) {
+#pragma unroll
+        for (int j = 0; j < G::VEC; j++)
+          if (g * G::VEC + j < V) push(to_f32(x[g * G::VEC + j]), g * G::VEC + j);
+      }
+    return;
+  }
+  for (int b = g0 + 32 * w; b < g1; b += kThreads) {
+    const int mine = b + l;
+    const bool want =
+        mine < g1 && mine * G::GROUP < V && top_key(gmax[mine], (uint32_t)(mine * G::GROUP)) > floor;
+    for (unsigned todo = __ballot_sync(kFull, want); todo; todo &= todo - 1) {
+      const int at = (b + __ffs(todo) - 1) * G::GROUP + l * G::VEC;
+      float v[G::VEC];
+      load_vec<T>(x, at, V, mis, v);
+#pragma unroll
+      for (int j = 0; j < G::VEC; j++) push(v[j], at + j);
+    }
+  }
+}
+// the row's k largest keys, in order, to sh.key[0 .. k)
+template <typename T>
+DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int k, TopShared& sh) {
+  const int ng = (V + group_size<T>(V) - 1) / group_size<T>(V);
+  if (threadIdx.x == 0) sh.count = sh.bits[0] = sh.bits[1] = 0;
+  __syncthreads();
+  // a value that at least k entries reach: the k-th largest maximum
+  unsigned long long floor = 0;
+  if (ng > k) {
+    constexpr int PER = kSmallVocab / Seg<T>::VEC / kThreads;  // as many groups as there can be, or more
+    static_assert(PER * kThreads >= (int)kMaxVocab / Seg<T>::GROUP, "every group has a place");
+    uint32_t v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int g = i * kThreads + threadIdx.x;
+      v[i] = g < ng ? (uint32_t)(top_key(gmax[g], 0) >> 32) : 0u;
+    }
+    const uint32_t t = kth_largest<uint32_t, PER>(v, k, sh);
+    floor = t ? ((unsigned long long)t << 32) - 1 : 0;
+  }
+  collect<T>(x, V, mis, gmax, 0, ng, floor, sh);
+  __syncthreads();
+  if (sh.count > kCand + kThreads) {
+    // too many entries reach it (ties, or a row in order): group by group in
+    // the order of their indices, cutting the list down as it fills, which
+    // raises the floor and passes over groups that cannot add to it
+    const int step = (kCand + kThreads - (int)DET_MAX_TOP) / group_size<T>(V);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (int g = 0; g < ng; g += step) {
+      collect<T>(x, V, mis, gmax, g, min(ng, g + step), floor, sh);
+      const unsigned long long t = cut_to(k, sh);
+      if (t) floor = t;
+    }
+  } else if (sh.count > kThreads) {
+    cut_to(k, sh);
+  }
+  __syncthreads();
+  // at most kThreads keys are left: each finds its rank
+  const int n = sh.count;
+  const unsigned long long mine = (int)threadIdx.x < n ? sh.key[threadIdx.x] : 0;
+  int rank = 0;
+  for (int i = 0; i < n; i++) rank += sh.key[i] > mine;
+  __syncthreads();
+  if ((int)threadIdx.x < n && rank < k) sh.key[rank] = mine;
+  __syncthreads();
+}
+
+// ---- clusters ------------------------------------------------------------------------
+DI uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+DI uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+DI void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+DI void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// *p of block `rank` of the cluster, p an address of one's own shared memory
+DI uint32_t remote(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+DI void store_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+
+// ---- forward ---------------------------------------------------------------------------
+// One cluster per row (of one block where there are rows enough): its warps
+// take segments in turn, their sums and group maxima go to block 0, which
+// joins them and writes the row's results.
+struct ForwardShared {
+  float m[kMaxSegs], s[kMaxSegs], w[kMaxSegs];
+  RowStats row;
+  ListShared list;
+  double dred[kThreads / 32];
+};
+template <typename T, bool TOP, bool SCALED>
+__global__ void __launch_bounds__(kThreads, 2)
+    forward_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, float* loss, ScoreOut o,
+                   float one) {
+  using G = Seg<T>;
+  __shared__ ForwardShared sh;
+  extern __shared__ float dyn[];  // TOP: group maxima, then a TopShared
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const int row = blockIdx.x / size, V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
+  const int nseg = (V + kSeg - 1) / kSeg, mis = misaligned(x);
+  const float inv_t = SCALED ? fdiv(1.0f, temp) : 1.0f;
+  if (size > 1) cluster_arrive();  // block 0 runs before anyone writes to it
+  bool first = size > 1;
+  for (int g = rank * (kThreads / 32) + w; g < nseg; g += size * (kThreads / 32)) {
+    float v[kPerLane];
+    load_segment<T>(x, g, V, mis, v);
+    float m = -INFINITY, gm = -INFINITY;
+    float lm[G::NV];
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) {
+      lm[i] = v[i * G::VEC];
+#pragma unroll
+      for (int j = 1; j < G::VEC; j++) lm[i] = fmaxf(lm[i], v[i * G::VEC + j]);
+      m = fmaxf(m, lm[i]);
+      if constexpr (TOP) {
+        const float r = redux_max(lm[i]);
+        if (l == i) gm = r;
+      }
+    }
+    m = redux_max(m);
+    const Sums r = segment_sums<SCALED>(v, m, inv_t, one);
+    if (first) cluster_wait();
+    first = false;
     if (l == 0) {
-      rs = r;
+      store_remote(remote(&sh.m[g], 0), r.m);
+      store_remote(remote(&sh.s[g], 0), r.s);
+      store_remote(remote(&sh.w[g], 0), r.s1);
+    }
+    if constexpr (TOP) {
+      if (V <= kSmallVocab) {
+#pragma unroll
+        for (int i = 0; i < G::NV; i++) store_remote(remote(&dyn[g * (kSeg / G::VEC) + i * 32 + l], 0), lm[i]);
+      } else if (l < G::NV) {
+        store_remote(remote(&dyn[g * G::NV + l], 0), gm);
+      }
+    }
+  }
+  if (size > 1) {
+    if (first) cluster_wait();
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  if (w == 0) {
+    const RowStats r = finish_row(join_segments(sh.m, sh.s, sh.w, nseg, inv_t, one));
+    if (l == 0) {
+      sh.row = r;
       if (o.stats) {
         float* st = o.stats + (size_t)row * 4;
-        st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = r.log_s;
+        st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = (float)r.log_s;
       }
       if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
     }
   }
   __syncthreads();
-  const RowStats r = rs;
+  const RowStats r = sh.row;
   const float nan = __int_as_float(0x7fffffff);
-  const double log_s = r.empty || r.bad ? 0.0 : log_det((double)r.s);
   if (loss) {
     bool some, bad;
-    const ListEntry e = teacher_entry(te, row, V, temp, one, lsh, &some, &bad);
+    const ListEntry e = teacher_entry(te, row, V, temp, one, sh.list, &some, &bad);
     double term = 0.0;
     if (e.id >= 0 && e.q > 0.0f) {
       const double z = (double)to_f32(x[e.id]);
-      const double logp = r.empty ? (double)-INFINITY : dsub(ddiv(dsub(z, (double)r.m), (double)temp), log_s);
+      const double logp = r.empty ? (double)-INFINITY : dsub(ddiv(dsub(z, (double)r.m), (double)temp), r.log_s);
       term = dmul((double)e.q, dsub(e.logq, logp));
     }
     term = warp_sum_d(term);
-    if (l == 0) dred[w] = term;
+    if (l == 0) sh.dred[w] = term;
     __syncthreads();
     if (threadIdx.x == 0) {
       double s = 0.0;
-      for (int i = 0; i < kThreads / 32; i++) s = dadd(s, dred[i]);
+      for (int i = 0; i < kThreads / 32; i++) s = dadd(s, sh.dred[i]);
       loss[row] = bad ? nan : !some ? 0.0f : r.bad ? nan : (float)s;
       if (bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
     }
     return;
   }
   if (threadIdx.x == 0) {
-    if (o.entropy) o.entropy[row] = r.bad ? nan : r.empty ? 0.0f : (float)dsub(log_s, ddiv((double)r.s1, (double)r.s));
+    if (o.entropy) {
+      o.entropy[row] = r.bad     ? nan
+                       : r.empty ? 0.0f
+                                 : (float)dsub(r.log_s, ddiv((double)r.s1, (double)r.s));
+    }
     if (o.logprob) {
       const long long t = load_id(tokens, id_bytes, row);
       float v;
       if (r.bad || t >= V) v = nan;
       else if (t < 0) v = 0.0f;
       else if (r.empty) v = -INFINITY;
-      else v = (float)dsub(dsub((double)to_f32(x[t]), (double)r.m), log_s);
+      else v = (float)dsub(dsub((double)to_f32(x[t]), (double)r.m), r.log_s);
       o.logprob[row] = v;
       if (t >= V && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
     }
   }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < o.top; k++) {
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-      const unsigned long long key = top_key(to_f32(x[i]), (uint32_t)i);
-      if (key < last && key > best) best = key;
-    }
-    for (int s = 16; s > 0; s >>= 1) best = max(best, __shfl_xor_sync(kFull, best, s));
-    __syncthreads();
-    if (l == 0) kred[w] = best;
-    __syncthreads();
-    best = 0;
-    for (int i = 0; i < kThreads / 32; i++) best = max(best, kred[i]);
-    last = best;
-    if (threadIdx.x == 0) {
-      const size_t at = (size_t)row * o.top + k;
-      if (o.top_ids) o.top_ids[at] = r.bad ? -1 : (int32_t)(0xffffffffu - (uint32_t)best);
+  if constexpr (TOP) {
+    TopShared& top = *reinterpret_cast<TopShared*>(dyn + (size_t)nseg * (kSeg / group_size<T>(V)));
+    if (!r.bad) top_list<T>(x, V, mis, dyn, o.top, top);
+    if ((int)threadIdx.x < o.top) {
+      const size_t at = (size_t)row * o.top + threadIdx.x;
+      const unsigned long long key = r.bad ? 0 : top.key[threadIdx.x];
+      if (o.top_ids) o.top_ids[at] = r.bad ? -1 : (int32_t)(0xffffffffu - (uint32_t)key);
       if (o.top_logprobs) {
         o.top_logprobs[at] = r.bad     ? nan
                              : r.empty ? -INFINITY
-                                       : (float)dsub(dsub((double)key_value(best), (double)r.m), log_s);
+                                       : (float)dsub(dsub((double)key_value(key), (double)r.m), r.log_s);
       }
     }
   }
@@ -499,11 +788,43 @@ cudaError_t by_dtype(int dtype, F f) {
   return cudaGetLastError();
 }
 
+// Blocks per row: enough for the GPU (two blocks of 8 warps per SM) while
+// every warp keeps a segment.
+int cluster_for(int n, int vocab) {
+  const int nseg = (vocab + kSeg - 1) / kSeg, sms = device_sms();
+  int c = 1;
+  while (c < 8 && (long long)n * c < 2 * sms && nseg > c * (kThreads / 32)) c *= 2;
+  return c;
+}
+template <typename T, bool TOP, bool SCALED>
+cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te,
+                       float temp, float* loss, const ScoreOut& o) {
+  const size_t smem = TOP ? groups_of<T>(L.vocab) * sizeof(float) + sizeof(TopShared) : 0;
+  if (cudaError_t e = raise_smem_cap((const void*)forward_kernel<T, TOP, SCALED>, smem)) return e;
+  const int c = cluster_for(L.n, L.vocab);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(L.n * c));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = c > 1;
+  return cudaLaunchKernelEx(&cfg, forward_kernel<T, TOP, SCALED>, L, tokens, id_bytes, te, temp, loss, o, 1.0f);
+}
 cudaError_t launch_forward(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
                            const Teacher& te, float temp, float* loss, const ScoreOut& o) {
-  return by_dtype(dtype, [&](auto t) {
-    forward_kernel<decltype(t)><<<L.n, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, loss, o, 1.0f);
+  cudaError_t e = cudaSuccess;
+  const cudaError_t last = by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    e = o.top         ? forward_as<T, true, false>(s, L, tokens, id_bytes, te, temp, loss, o)
+        : temp == 1.0f ? forward_as<T, false, false>(s, L, tokens, id_bytes, te, temp, loss, o)
+                       : forward_as<T, false, true>(s, L, tokens, id_bytes, te, temp, loss, o);
   });
+  return e ? e : last;
 }
 cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
                         const Teacher& te, float temp, const GradIn& in, void* out, unsigned long long out_ld) {
