@@ -184,19 +184,45 @@ DI uint4 shifted(uint4 a, uint4 b, int bytes) {
 // VEC entries from entry `at` of a row; what is past its end is -inf.  Only
 // 16-byte granules that lie in the row as a whole are loaded as such: a row
 // that starts `mis` entries into a granule takes two of them per vector.
-template <typename T>
-DI void load_vec(const T* __restrict__ row, int at, int V, int mis, float* v) {
+// RO: nothing writes the row while the kernel runs.
+template <bool RO>
+DI uint4 load16(const uint4* p) {
+  if constexpr (RO) return __ldg(p);
+  else return *p;
+}
+template <typename T, bool RO = true>
+DI void load_vec(const T* row, int at, int V, int mis, float* v) {
   constexpr int VEC = Seg<T>::VEC;
   const T* p = row + at;
-  if (mis == 0 && at + VEC <= V) {
-    unpack_vec<T>(__ldg(reinterpret_cast<const uint4*>(p)), v);
+  if (mis == 0 && at >= 0 && at + VEC <= V) {
+    unpack_vec<T>(load16<RO>(reinterpret_cast<const uint4*>(p)), v);
   } else if (mis != 0 && at >= mis && at - mis + 2 * VEC <= V) {
     const uint4* q = reinterpret_cast<const uint4*>(p - mis);
-    unpack_vec<T>(shifted(__ldg(q), __ldg(q + 1), mis * (int)sizeof(T)), v);
+    unpack_vec<T>(shifted(load16<RO>(q), load16<RO>(q + 1), mis * (int)sizeof(T)), v);
   } else {
 #pragma unroll
-    for (int j = 0; j < VEC; j++) v[j] = at + j < V ? to_f32(p[j]) : -INFINITY;
+    for (int j = 0; j < VEC; j++) v[j] = at + j >= 0 && at + j < V ? to_f32(p[j]) : -INFINITY;
   }
+}
+template <typename T>
+DI uint4 pack_vec(const float* v) {
+  uint32_t w[4];
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        memcpy(&w[i], &h, 4);
+      } else {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        memcpy(&w[i], &h, 4);
+      }
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T>
 DI int misaligned(const T* row) {
@@ -692,89 +718,143 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// ---- gradient ----------------------------------------------------------------------
-// dx_j = exp(d_j) (a + b d_j) + (what the row's own tokens add): one block per
-// row.  `out` may be the logits themselves.
+// ---- gradient --------------------------------------------------------------------------
+// dx_j = exp(d_j) (a + b d_j) + (what the row's own tokens add).  `as`, `bs`
+// are a and b over S.
 struct GradIn {
   const float *stats, *g, *gh;  // g: of logprob or of the loss; gh: of the entropy, or null
 };
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    grad_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, T* out,
-                unsigned long long out_ld, float one_) {
-  __shared__ ListShared lsh;
-  __shared__ int ids[DET_MAX_TOP];
-  __shared__ float add[DET_MAX_TOP];
-  const int row = blockIdx.x, V = L.vocab;
-  const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
-  T* y = out + (size_t)row * out_ld;
-  const float *st = in.stats + (size_t)row * 4, nan = __int_as_float(0x7fffffff);
-  const float inv_t = fdiv(1.0f, temp);
-  const float m = st[0], s = st[1], s1 = st[2];
+struct RowGrad {
+  float base, inv_t, as, bs;  // base: -m
+  bool zero;                  // nothing but zeros
+};
+struct GradShared {
+  ListShared list;
+  int id[DET_MAX_TOP];
+  float add[DET_MAX_TOP];
+};
+// gradients of a pair of entries
+template <bool ENTROPY, bool SCALED>
+DI f2 grad2(f2 x, const RowGrad& r, f2 one) {
+  f2 d = add2(x, pk(r.base, r.base));
+  if constexpr (SCALED) d = mul2(d, pk(r.inv_t, r.inv_t));
+  const Exp2 e = exp2_lanes(d, one);
+  if constexpr (ENTROPY) return mul2(e.e, addp(mul2(e.d, pk(r.bs, r.bs)), one, pk(r.as, r.as)));
+  return mul2(e.e, pk(r.as, r.as));
+}
+// the row's coefficients, and in sh what its tokens add: id[i] (or -1) and
+// add[i] for i < the returned count.  Ends with a barrier.
+DI int row_grad(int row, int V, const void* tokens, int id_bytes, const Teacher& te, float temp, const GradIn& in,
+                float m, float s, float s1, float one, GradShared& sh, RowGrad& r) {
+  const float nan = __int_as_float(0x7fffffff);
   const bool empty = m == -INFINITY;
   const float g = in.g ? in.g[row] : 0.0f;
   float a, b = 0.0f;
-  int k = 0;
+  bool blank = false;
+  int k = 1;
   if (te.k) {
     bool some, bad;
-    const ListEntry e = teacher_entry(te, row, V, temp, one_, lsh, &some, &bad);
-    const float gt = fdiv(g, temp);
-    a = bad ? nan : !some || empty ? 0.0f : gt;
-    if (!some && !bad) b = nan;  // marks a row without a list: zeros whatever its logits
-    if (threadIdx.x < te.k) {
-      ids[threadIdx.x] = e.id;
-      add[threadIdx.x] = e.q;
+    const ListEntry e = teacher_entry(te, row, V, temp, one, sh.list, &some, &bad);
+    blank = !some && !bad;
+    a = bad ? nan : fdiv(g, temp);
+    k = te.k;
+    if ((int)threadIdx.x < k) {
+      sh.id[threadIdx.x] = e.id;
+      sh.add[threadIdx.x] = e.q;
     }
     __syncthreads();
     // an id that is listed twice: its first entry takes the sum, in order
     float sum = 0.0f;
-    if (threadIdx.x < te.k && e.id >= 0) {
-      bool first = true;
-      for (int i = 0; i < te.k; i++)
-        if (ids[i] == e.id) {
+    bool first = true;
+    if ((int)threadIdx.x < k && e.id >= 0)
+      for (int i = 0; i < k; i++)
+        if (sh.id[i] == e.id) {
           if (i < (int)threadIdx.x) first = false;
-          sum = fadd(sum, add[i]);
+          sum = fadd(sum, sh.add[i]);
         }
-      if (!first) sum = -1.0f;
-    }
     __syncthreads();
-    if (threadIdx.x < te.k) {
-      if (sum < 0.0f) ids[threadIdx.x] = -1;
-      add[threadIdx.x] = fmul(-a, sum);
+    if ((int)threadIdx.x < k) {
+      if (!first) sh.id[threadIdx.x] = -1;
+      sh.add[threadIdx.x] = fmul(-a, sum);
     }
-    k = te.k;
   } else {
     const float gh = in.gh ? in.gh[row] : 0.0f;
     const long long t = in.g ? load_id(tokens, id_bytes, row) : -1;
     const float gl = t < 0 ? 0.0f : t >= V ? nan : g;
-    a = empty ? 0.0f : fadd(-gl, fmul(gh, fdiv(s1, s)));
-    b = empty ? 0.0f : -gh;
+    a = fadd(-gl, fmul(gh, fdiv(s1, s)));
+    b = -gh;
     if (threadIdx.x == 0) {
-      ids[0] = t >= 0 && t < V ? (int)t : -1;
-      add[0] = empty ? 0.0f : gl;
+      sh.id[0] = t >= 0 && t < V ? (int)t : -1;
+      sh.add[0] = gl;
     }
-    k = 1;
   }
-  const bool blank = te.k && !(b == b);
-  if (blank) b = 0.0f;
+  const float inv_s = fdiv(1.0f, s);
+  r.zero = blank || empty;
+  r.base = -m;
+  r.inv_t = fdiv(1.0f, temp);
+  r.as = fmul(a, inv_s);
+  r.bs = fmul(b, inv_s);
   __syncthreads();
-  const float base = empty ? 0.0f : -m, inv_s = empty ? 0.0f : fdiv(1.0f, s);
-  const float as = fmul(a, inv_s), bs = fmul(b, inv_s);
+  return k;
+}
+
+// Blocks (blockIdx.x) of a row (blockIdx.y + row0) take `per` of its 16-byte
+// vectors each; a vector is one of the gradient's, so that stores are whole
+// wherever the row starts.  `out` may be the logits themselves.
+constexpr int kGradUnroll = 4;
+template <typename T, bool ENTROPY, bool SCALED>
+__global__ void __launch_bounds__(kThreads)
+    grad_kernel(Logits L, int row0, int per, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in,
+                T* out, unsigned long long out_ld, float one_) {
+  constexpr int VEC = Seg<T>::VEC;
+  __shared__ GradShared sh;
+  const int row = row0 + blockIdx.y, V = L.vocab;
+  const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
+  T* y = out + (size_t)row * out_ld;
+  const float* st = in.stats + (size_t)row * 4;
+  RowGrad r;
+  const int k = row_grad(row, V, tokens, id_bytes, te, temp, in, st[0], st[1], st[2], one_, sh, r);
   const f2 one = pk(one_, one_);
-  auto grad = [&](float v) {
-    const Exp2 e = exp2_lanes(mul2(add2(pk(v, v), pk(base, base)), pk(inv_t, inv_t)), one);
-    const f2 c = b == 0.0f ? pk(as, as) : addp(mul2(e.d, pk(bs, bs)), one, pk(as, as));
-    const float r = un(mul2(e.e, c)).x;
-    return blank || empty ? 0.0f : r;
-  };
+  const int my = misaligned(y), mis = (misaligned(x) - my) & (VEC - 1);
+  const int nvec = (V + my + VEC - 1) / VEC;
+  const int q0 = blockIdx.x * per, q1 = min(nvec, q0 + per);
   // the values at the row's own tokens, before `out` may overwrite them
+  const int id = (int)threadIdx.x < k ? sh.id[threadIdx.x] : -1;
+  const bool patch = id >= 0 && id >= q0 * VEC - my && id < q1 * VEC - my && !r.zero;
   float mine = 0.0f;
-  const int id = threadIdx.x < k ? ids[threadIdx.x] : -1;
-  if (id >= 0) mine = fadd(grad(to_f32(x[id])), add[threadIdx.x]);
+  if (patch) {
+    const float v = to_f32(x[id]);
+    mine = fadd(un(grad2<ENTROPY, SCALED>(pk(v, v), r, one)).x, sh.add[threadIdx.x]);
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < V; i += kThreads) y[i] = from_f32<T>(grad(to_f32(x[i])));
+  for (int q = q0 + threadIdx.x; q < q1; q += kThreads * kGradUnroll) {
+    float v[kGradUnroll][VEC];
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; u++) {
+      const int at = (q + u * kThreads) * VEC - my;
+      if (q + u * kThreads < q1) load_vec<T, false>(x, at, V, mis, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kGradUnroll; u++) {
+      const int at = (q + u * kThreads) * VEC - my;
+      if (q + u * kThreads >= q1) continue;
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        const float2 gr = un(grad2<ENTROPY, SCALED>(pk(v[u][j], v[u][j + 1]), r, one));
+        v[u][j] = r.zero ? 0.0f : gr.x;
+        v[u][j + 1] = r.zero ? 0.0f : gr.y;
+      }
+      if (at >= 0 && at + VEC <= V) {
+        *reinterpret_cast<uint4*>(y + at) = pack_vec<T>(v[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          if (at + j >= 0 && at + j < V) y[at + j] = from_f32<T>(v[u][j]);
+      }
+    }
+  }
   __syncthreads();
-  if (id >= 0 && !blank && !empty) y[id] = from_f32<T>(mine);
+  if (patch) y[id] = from_f32<T>(mine);
 }
 
 // ---- launches --------------------------------------------------------------------
@@ -826,12 +906,32 @@ cudaError_t launch_forward(cudaStream_t s, int dtype, const Logits& L, const voi
   });
   return e ? e : last;
 }
+template <typename T, bool ENTROPY, bool SCALED>
+cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
+                    const GradIn& in, void* out, unsigned long long out_ld) {
+  constexpr int VEC = Seg<T>::VEC;
+  const int nvec = (L.vocab + VEC - 1) / VEC + 1;  // one more where a row starts inside a vector
+  const int step = kThreads * kGradUnroll;
+  int per = 4 * step;
+  while (per > step && (long long)L.n * ((nvec + per - 1) / per) < 8 * device_sms()) per -= step;
+  const int blocks = (nvec + per - 1) / per;
+  for (int r = 0; r < L.n; r += 65535) {
+    grad_kernel<T, ENTROPY, SCALED><<<dim3(blocks, L.n - r < 65535 ? L.n - r : 65535), kThreads, 0, s>>>(
+        L, r, per, tokens, id_bytes, te, temp, in, static_cast<T*>(out), out_ld, 1.0f);
+    if (cudaError_t e = cudaGetLastError()) return e;
+  }
+  return cudaSuccess;
+}
 cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
                         const Teacher& te, float temp, const GradIn& in, void* out, unsigned long long out_ld) {
-  return by_dtype(dtype, [&](auto t) {
+  cudaError_t e = cudaSuccess;
+  const cudaError_t last = by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    grad_kernel<T><<<L.n, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, static_cast<T*>(out), out_ld, 1.0f);
+    e = in.gh           ? grad_as<T, true, false>(s, L, tokens, id_bytes, te, temp, in, out, out_ld)
+        : temp == 1.0f ? grad_as<T, false, false>(s, L, tokens, id_bytes, te, temp, in, out, out_ld)
+                       : grad_as<T, false, true>(s, L, tokens, id_bytes, te, temp, in, out, out_ld);
   });
+  return e ? e : last;
 }
 
 // ---- argument checks ----------------------------------------------------------------

@@ -470,6 +470,22 @@ def test_rows_far_apart(env):
                        sc.distill_step(x, f.top_ids, f.top_logprobs, one)[1])
 
 
+def test_more_rows_than_a_grid_dimension_holds(env):
+    _, torch, sc = env
+    n, vocab = 66001, 19
+    x, tokens, g = make(torch, n, vocab, torch.float32, 2)
+    one = torch.randn(n, generator=g, device="cuda")
+    fwd = sc.token_scores(x, tokens, top=2)
+    _, lp, h, tol_lp, tol_h = scores_ref(torch, x.double(), tokens)
+    close(torch, fwd.logprob, lp, tol_lp)
+    close(torch, fwd.entropy, h, tol_h)
+    ref, tol = scores_grad_ref(torch, x.double(), tokens, one, one, x.dtype)
+    close(torch, sc.token_scores_grad(x, tokens, fwd.stats, one, one), ref, tol)
+    close(torch, sc.token_scores_step(x, tokens, one, one)[1], ref, tol)
+    ref, tol = distill_grad_ref(torch, x.double(), fwd.top_ids.long(), fwd.top_logprobs, 1.0, one, x.dtype)
+    close(torch, sc.distill_step(x, fwd.top_ids, fwd.top_logprobs, one)[1], ref, tol)
+
+
 def test_one_row_many_times(env):
     """An expanded row (stride 0) is read as any other."""
     _, torch, sc = env
