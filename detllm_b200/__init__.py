@@ -111,10 +111,11 @@ def lib():
             "det_symbol_ranges_noalloc": (I, [P, U32, U32, P, I, P, P]),
             "det_token_scores": (I, [P, P, P, U32, U32, P, P, P, P]),
             "det_distill_loss": (I, [P, P, U32, P, P, U32, F32, P]),
-            "det_token_scores_device": (I, [P, I, U32, U32, U64, P, I, U32, P, P, P, P, P, P, P]),
+            "det_scores_workspace": (SZ, [I, U32, U32, U32]),
+            "det_token_scores_device": (I, [P, I, U32, U32, U64, P, I, U32, P, P, P, P, P, P, P, SZ, P]),
             "det_token_scores_grad_device": (I, [P, I, U32, U32, U64, P, I, P, P, P, P, U64, P]),
             "det_token_scores_step_device": (I, [P, I, U32, U32, U64, P, I, P, P, P, P, P, P, U64, P, P]),
-            "det_distill_loss_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P]),
+            "det_distill_loss_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P, SZ, P]),
             "det_distill_grad_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, U64, P]),
             "det_distill_step_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P, U64, P, P]),
             "det_tp_exchange_timeout_selftest": (I, [I]),

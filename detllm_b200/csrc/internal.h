@@ -201,12 +201,15 @@ cudaError_t launch_cdf_ranges(const Launch& L, const float* e, const float* z, i
                               const uint32_t* rows, const uint32_t* symbols, int n, uint64_t* out3);
 // Token scores and distillation on a session's f32 logits (scoring.cu): row
 // rows[i] for output i.  tokens as int32 (negative: ignored); top list arrays
-// may be null when top is 0; lists are k entries, int32 ids and f32 values
+// may be null when top is 0; lists are k entries, int32 ids and f32 values.
+// workspace: device memory, 16-byte aligned, scores_workspace_bytes
 cudaError_t launch_token_scores(const Launch& L, const float* logits, int V, const uint32_t* rows,
                                 const uint32_t* tokens, int n, int top, float* logprob, float* entropy,
-                                int32_t* top_ids, float* top_logprobs);
+                                int32_t* top_ids, float* top_logprobs, void* workspace);
 cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, const uint32_t* rows, int n,
-                                const int32_t* ids, const float* teacher, int k, float temperature, float* loss);
+                                const int32_t* ids, const float* teacher, int k, float temperature, float* loss,
+                                void* workspace);
+size_t scores_workspace_bytes(int n, int V, int top);  // of the two
 cudaError_t launch_expf(cudaStream_t st, const float* x, float* y, long long n);
 // GGUF tensor bytes (in device memory) -> device layouts (repack.cu); a
 // non-finite scale or value sets ERRF_NONFINITE in *err

@@ -22,6 +22,10 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <map>
+#include <mutex>
+#include <set>
+#include <tuple>
 #include <type_traits>
 
 #include "../../include/detgpu.h"
@@ -35,7 +39,7 @@ constexpr int kSeg = 2048;                       // entries per segment
 constexpr int kPerLane = kSeg / 32;              // entries per lane of a segment
 constexpr uint32_t kMaxVocab = 1u << 18;         // as the CDF's alphabet
 constexpr int kMaxSegs = (int)(kMaxVocab / kSeg);
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kFull = 0xffffffffu;
 
 // ---- packed f32 pairs ----------------------------------------------------------
@@ -76,39 +80,68 @@ DI float max_nan(float a, float b) {  // NaN if either is
   return r;
 }
 
-// exp(d) for d <= 0, two at a time: d = k ln 2 + r with |r| <= ln 2 / 2 (a
-// two-part ln 2 whose parts times k are exact), exp(r) by a degree-5 minimax
-// polynomial 1 + r + r^2 q(r) (relative error 1.06e-7), 2^k added to the
-// exponent field.  Below kExpLow the result is +0 (the exponent field goes
-// negative there and the integer maximum clears it); it is within 3.1 * 2^-24
-// of exp(d) for d >= -87.  NaN gives an unspecified number: callers keep d,
-// which stays NaN, beside it.
-constexpr float kExpLow = -88.13f;  // k = -127, r = -0.10
-struct Exp2 {
-  f2 e, d;  // exp, and the argument as clamped
+// 2^y for y <= 0, two at a time, by Tang's table-driven method: y = k + i/32 +
+// f with |f| <= 1/64 (a rounding to a multiple of 1/32 by adding 1.5 * 2^18),
+// 2^f by a degree-2 minimax polynomial (relative error 0.9 * 2^-24), 2^(i/32)
+// from a table of 32 that a warp holds one entry per lane and reads with a
+// shuffle (no two lanes conflict), 2^k added to the entry's exponent field.
+// 13 rounded f32 operations per entry of a row with its two sums, against 19
+// for a degree-5 polynomial on |f| <= 1/2: the f32 pipe bounds the passes over
+// 16-bit logits, while the shuffle and the integer operations run beside it.
+// Within 3.8 * 2^-24 of 2^y for y >= -126.  At kYLow the result is +0 (the
+// exponent field goes negative there and the integer maximum clears it).  NaN
+// gives an unspecified number: callers keep y, which stays NaN, beside it.
+constexpr float kYLow = -127.5f;
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147182f;
+// bits of 2^(i/32), less i << 18: adding (32 k + i) << 18 leaves 2^(k + i/32)
+static __device__ const uint32_t kExpTable[32] = {
+    0x3f800000u, 0x3f7ecd87u, 0x3f7daac3u, 0x3f7c980fu, 0x3f7b95c2u, 0x3f7aa43au, 0x3f79c3d3u, 0x3f78f4f0u,
+    0x3f7837f0u, 0x3f778d3au, 0x3f76f532u, 0x3f767043u, 0x3f75fed7u, 0x3f75a15bu, 0x3f75583fu, 0x3f7523f6u,
+    0x3f7504f3u, 0x3f74fbafu, 0x3f7508a4u, 0x3f752c4du, 0x3f75672au, 0x3f75b9beu, 0x3f76248cu, 0x3f76a81eu,
+    0x3f7744fdu, 0x3f77fbb8u, 0x3f78ccdfu, 0x3f79b907u, 0x3f7ac0c7u, 0x3f7be4bau, 0x3f7d257du, 0x3f7e83b3u,
 };
-DI Exp2 exp2_lanes(f2 d, f2 one) {
-  float2 c = un(d);
-  c.x = max_nan(c.x, kExpLow);
-  c.y = max_nan(c.y, kExpLow);
-  d = pk(c.x, c.y);
-  const f2 magic = pk(12582912.0f, 12582912.0f), nmagic = pk(-12582912.0f, -12582912.0f);
-  const f2 z = addp(mul2(d, pk(1.44269504f, 1.44269504f)), one, magic);
-  const f2 k = add2(z, nmagic);
-  const f2 nhi = pk(-0.693145751953125f, -0.693145751953125f);
-  const f2 nlo = pk(-1.4286197256296873e-06f, -1.4286197256296873e-06f);
-  // k has 7 bits and the parts of ln 2 have 15: exact products
-  const f2 r = fma2(k, nlo, fma2(k, nhi, d));
-  f2 q = addp(mul2(pk(0.008312501f, 0.008312501f), r), one, pk(0.04189033f, 0.04189033f));
-  q = addp(mul2(q, r), one, pk(0.16667116f, 0.16667116f));
-  q = addp(mul2(q, r), one, pk(0.4999923f, 0.4999923f));
-  const f2 p = add2(addp(mul2(q, mul2(r, r)), one, r), pk(1.0f, 1.0f));
-  const float2 pf = un(p), zf = un(z);
-  const int ex = max(__float_as_int(pf.x) + (__float_as_int(zf.x) << 23), 0);
-  const int ey = max(__float_as_int(pf.y) + (__float_as_int(zf.y) << 23), 0);
-  return {pk(__int_as_float(ex), __int_as_float(ey)), d};
+struct Exp2 {
+  f2 e, y;  // 2^y, and y as clamped
+};
+struct ExpParts {
+  f2 z, p, y;  // magic + (32 k + i) / 32, 2^f, the clamped argument
+};
+template <bool CLAMP>
+DI ExpParts exp_parts(f2 y, f2 one) {
+  if constexpr (CLAMP) {
+    float2 c = un(y);
+    c.x = max_nan(c.x, kYLow);
+    c.y = max_nan(c.y, kYLow);
+    y = pk(c.x, c.y);
+  }
+  const f2 magic = pk(393216.0f, 393216.0f), neg = pk(-1.0f, -1.0f);
+  const f2 z = addp(y, one, magic);  // y may come straight from a multiply
+  const f2 f = addp(y, one, fma2(z, neg, magic));  // magic - z: an exact multiply by -1
+  const f2 q = addp(mul2(pk(0.24022649f, 0.24022649f), f), one, pk(0.6931573f, 0.6931573f));
+  return {z, addp(mul2(q, f), one, pk(1.0f, 1.0f)), y};
 }
-DI float exp1(float d, float one) { return un(exp2_lanes(pk(d, d), pk(one, one)).e).x; }
+template <bool CLAMP>
+DI float exp_scale(uint32_t entry, float z) {
+  const int b = (int)(entry + (__float_as_uint(z) << 18));
+  return __int_as_float(CLAMP ? max(b, 0) : b);
+}
+// every lane of the warp takes part; `table`: the lane's entry.  Without CLAMP
+// every y that is a number has to be >= kYSafe; the bits are the same.
+constexpr float kYSafe = -126.0f;
+template <bool CLAMP>
+DI Exp2 exp2_warp(f2 y, uint32_t table, f2 one) {
+  const ExpParts t = exp_parts<CLAMP>(y, one);
+  const float2 z = un(t.z);
+  const uint32_t ax = __shfl_sync(kFull, table, __float_as_int(z.x));
+  const uint32_t ay = __shfl_sync(kFull, table, __float_as_int(z.y));
+  return {mul2(pk(exp_scale<CLAMP>(ax, z.x), exp_scale<CLAMP>(ay, z.y)), t.p), t.y};
+}
+// one value, any lanes; the same bits
+DI float exp2_one(float y, float one) {
+  const ExpParts t = exp_parts<true>(pk(y, y), pk(one, one));
+  const float z = un(t.z).x;
+  return fmul(exp_scale<true>(kExpTable[__float_as_uint(z) & 31], z), un(t.p).x);
+}
 
 // ---- element types ---------------------------------------------------------------
 template <typename T>
@@ -151,8 +184,8 @@ DI void unpack_vec(uint4 w, float* v) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        v[2 * i] = __uint_as_float(__byte_perm(u[i], 0, 0x1044));
+        v[2 * i + 1] = __uint_as_float(__byte_perm(u[i], 0, 0x3244));
       } else {
         __half2 h;
         memcpy(&h, &u[i], 4);
@@ -228,25 +261,80 @@ template <typename T>
 DI int misaligned(const T* row) {
   return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
 }
+// A warp's segment on its way: its 16-byte granules (one more where the row
+// starts inside one) are copied to shared memory asynchronously, so the next
+// segment is fetched while this one is in registers.  What lies past the
+// row's end is -inf there.
 template <typename T>
-DI void load_segment(const T* __restrict__ row, int g, int V, int mis, float (&v)[kPerLane]) {
+constexpr int kStageBytes = kSeg * (int)sizeof(T) + 16;
+template <typename T>
+DI void stage_granule(uint32_t to, const T* row, int at, int V) {
+  constexpr int VEC = Seg<T>::VEC;
+  if (at >= 0 && at + VEC <= V) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
+  } else {
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) v[j] = at + j >= 0 && at + j < V ? to_f32(row[at + j]) : -INFINITY;
+    const uint4 w = pack_vec<T>(v);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+  }
+}
+template <typename T>
+DI void stage_issue(const void* buf, const T* row, int g, int V) {
   using G = Seg<T>;
-  const int base = g * kSeg + (threadIdx.x & 31) * G::VEC;
-  if (mis == 0 && (g + 1) * kSeg <= V) {
-    const uint4* p = reinterpret_cast<const uint4*>(row + base);
-    uint4 w[G::NV];
+  const int l = threadIdx.x & 31, mis = misaligned(row), first = g * kSeg - mis;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(buf) + 16 * l;
+  if (first >= 0 && first + kSeg + (mis ? G::VEC : 0) <= V) {  // no granule reaches out of the row
+    const T* p = row + first + l * G::VEC;
 #pragma unroll
-    for (int i = 0; i < G::NV; i++) w[i] = __ldg(p + 32 * i);
+    for (int i = 0; i < G::NV; i++)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * i), "l"(p + i * G::GROUP) : "memory");
+    if (mis != 0 && l == 0)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * G::NV), "l"(p + kSeg) : "memory");
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < G::NV; i++) stage_granule<T>(to + 512 * i, row, first + (32 * i + l) * G::VEC, V);
+    if (mis != 0 && l == 0) stage_granule<T>(to + 512 * G::NV, row, first + kSeg, V);
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// waits for the warp's segment and takes it; the buffer is free afterwards
+template <typename T>
+DI void stage_take(const void* buf, int mis, uint4 (&v)[Seg<T>::NV]) {
+  using G = Seg<T>;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+  const uint4* w = static_cast<const uint4*>(buf) + (threadIdx.x & 31);
+  if (mis == 0) {
 #pragma unroll
-    for (int i = 0; i < G::NV; i++) unpack_vec<T>(w[i], v + i * G::VEC);
+    for (int i = 0; i < G::NV; i++) v[i] = w[32 * i];
   } else {
 #pragma unroll
-    for (int i = 0; i < G::NV; i++) load_vec<T>(row, base + i * G::GROUP, V, mis, v + i * G::VEC);
+    for (int i = 0; i < G::NV; i++) v[i] = shifted(w[32 * i], w[32 * i + 1], mis * (int)sizeof(T));
+  }
+  __syncwarp();
+}
+// largest and smallest entry of a vector; NaN loses against a number
+template <typename T>
+DI void vec_range(uint4 w, float& hi, float& lo) {
+  if constexpr (std::is_same_v<T, float>) {
+    const float a = __uint_as_float(w.x), b = __uint_as_float(w.y), c = __uint_as_float(w.z), d = __uint_as_float(w.w);
+    hi = fmaxf(fmaxf(a, b), fmaxf(c, d));
+    lo = fminf(fminf(a, b), fminf(c, d));
+  } else {
+    using P = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    P p[4];
+    memcpy(p, &w, 16);
+    const P h = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    const P l = __hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3]));
+    hi = to_f32(__hmax(h.x, h.y));
+    lo = to_f32(__hmin(l.x, l.y));
   }
 }
 
 struct Sums {
-  float m, s, s1;
+  float m, s, w;  // maximum, sum of 2^y, sum of 2^y y, with y = (x - m) log2(e) / T
 };
 
 DI float warp_max(float v) {
@@ -257,29 +345,66 @@ DI float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fadd(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
+// the sum of s in lanes 0 .. 15, of w in lanes 16 .. 31
+DI float warp_sum2(float s, float w) {
+  const bool low = (threadIdx.x & 16) == 0;
+  float v = fadd(low ? s : w, __shfl_xor_sync(kFull, low ? w : s, 16));
+  for (int o = 8; o > 0; o >>= 1) v = fadd(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
 DI double warp_sum_d(double v) {
   for (int o = 16; o > 0; o >>= 1) v = dadd(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
 
-// maximum, sum of exp((x - m) / T) and the same weighted by (x - m) / T over
-// one segment's 64 entries per lane; a NaN or +inf anywhere leaves s1 NaN.
-// `m`: the segment's maximum.
-template <bool SCALED>
-DI Sums segment_sums(const float (&x)[kPerLane], float m, float inv_t, float one_) {
+// a segment's sums s (in lanes 0 .. 15) and w (in lanes 16 .. 31), of the lanes'
+// vectors v with maximum m; a NaN or +inf anywhere leaves w NaN.  Quarters of
+// the segment from `entries` on are all -inf and add nothing: they are passed
+// over.  KEEP: e becomes 2^y.
+template <typename T, bool KEEP, bool CLAMP>
+DI float sum_segment(const uint4 (&v)[Seg<T>::NV], int entries, float m, float c, uint32_t table, float one_,
+                     float* e) {
+  using G = Seg<T>;
   const float base = m == -INFINITY ? 0.0f : -m;
-  const f2 nm = pk(base, base), one = pk(one_, one_), it = pk(inv_t, inv_t);
+  const f2 nm = pk(base, base), one = pk(one_, one_), cc = pk(c, c);
   f2 s[2] = {0, 0}, w[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < kPerLane / 2; i++) {
-    f2 d = add2(pk(x[2 * i], x[2 * i + 1]), nm);
-    if constexpr (SCALED) d = mul2(d, it);
-    const Exp2 e = exp2_lanes(d, one);
-    s[i & 1] = add2(s[i & 1], e.e);
-    w[i & 1] = addp(mul2(e.e, e.d), one, w[i & 1]);
+  for (int q = 0; q < 4; q++) {
+    if (q * (kSeg / 4) >= entries) {
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < kPerLane / 4; i++) e[q * (kPerLane / 4) + i] = 0.0f;
+      }
+      continue;
+    }
+#pragma unroll
+    for (int i = q * (G::NV / 4); i < (q + 1) * (G::NV / 4); i++) {
+      float x[G::VEC];
+      unpack_vec<T>(v[i], x);
+#pragma unroll
+      for (int j = 0; j < G::VEC / 2; j++) {
+        const Exp2 t = exp2_warp<CLAMP>(mul2(add2(pk(x[2 * j], x[2 * j + 1]), nm), cc), table, one);
+        s[j & 1] = add2(s[j & 1], t.e);
+        w[j & 1] = addp(mul2(t.e, t.y), one, w[j & 1]);
+        if constexpr (KEEP) {
+          const float2 k = un(t.e);
+          e[i * G::VEC + 2 * j] = k.x;
+          e[i * G::VEC + 2 * j + 1] = k.y;
+        }
+      }
+    }
   }
   const float2 sp = un(add2(s[0], s[1])), wp = un(add2(w[0], w[1]));
-  return {m, warp_sum(fadd(sp.x, sp.y)), warp_sum(fadd(wp.x, wp.y))};
+  return warp_sum2(fadd(sp.x, sp.y), fadd(wp.x, wp.y));
+}
+// `low`: the smallest entry.  Where no entry is so far below the maximum that
+// its power has to be cleared, the clamp and the clearing are left out (4
+// integer-pipe operations of 23 per pair of entries).
+template <typename T, bool KEEP>
+DI float segment_sums(const uint4 (&v)[Seg<T>::NV], int entries, float m, float low, float c, uint32_t table,
+                      float one, float* e) {
+  if (fmul(fsub(low, m), c) >= kYSafe) return sum_segment<T, KEEP, false>(v, entries, m, c, table, one, e);
+  return sum_segment<T, KEEP, true>(v, entries, m, c, table, one, e);
 }
 DI float redux_max(float v) {  // of the warp; a NaN loses against a number
   float r;
@@ -287,39 +412,59 @@ DI float redux_max(float v) {  // of the warp; a NaN loses against a number
   return r;
 }
 
-// joins a row's segments (one warp; the result in every lane)
-DI Sums join_segments(const float* sm, const float* ss, const float* sw, int nseg, float inv_t, float one) {
+DI float redux_min(float v) {
+  float r;
+  asm volatile("redux.sync.min.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "r"(kFull));
+  return r;
+}
+
+// y of a segment's maximum under the row's
+DI float segment_y(float ms, float m, float c) {
+  return ms == -INFINITY ? kYLow : fmaxf(fmul(fsub(ms, m), c), kYLow);
+}
+// joins a row's segments (one warp; the result in every lane): at(i) gives
+// segment i's sums
+template <typename F>
+DI Sums join_segments(F at, int nseg, float c, float one) {
   const int l = threadIdx.x & 31;
+  Sums t[kMaxSegs / 32];
   float m = -INFINITY;
-  for (int i = l; i < nseg; i += 32) m = fmaxf(m, sm[i]);
-  m = warp_max(m);
+#pragma unroll
+  for (int i = 0; i < kMaxSegs / 32; i++) {
+    t[i] = 32 * i + l < nseg ? at(32 * i + l) : Sums{-INFINITY, 0.0f, 0.0f};
+    m = fmaxf(m, t[i].m);
+  }
+  m = redux_max(m);
   float s = 0.0f, w = 0.0f;
-  for (int i = l; i < nseg; i += 32) {
-    const bool empty = sm[i] == -INFINITY;
-    const float d = empty ? kExpLow : fmaxf(fmul(fsub(sm[i], m), inv_t), kExpLow);
-    const float f = exp1(d, one);
-    s = fadd(s, fmul(f, ss[i]));
-    // sum of exp(d_j + d) (d_j + d) = f (S1 + d S); NaN stays NaN
-    w = fadd(w, fmul(f, fadd(sw[i], fmul(d, ss[i]))));
+#pragma unroll
+  for (int i = 0; i < kMaxSegs / 32; i++) {
+    if (32 * i >= nseg) break;
+    const float y = segment_y(t[i].m, m, c);
+    const float f = exp2_one(y, one);
+    s = fadd(s, fmul(f, t[i].s));
+    // sum of 2^(y_j + y) (y_j + y) = f (w + y s); NaN stays NaN
+    w = fadd(w, fmul(f, fadd(t[i].w, fmul(y, t[i].s))));
   }
   return {m, warp_sum(s), warp_sum(w)};
 }
 
 struct RowStats {
   float m, s, s1;
-  double log_s;
   bool empty, bad;
 };
 DI RowStats finish_row(const Sums& r) {
   RowStats t;
-  t.bad = !(r.s1 == r.s1) || r.m == INFINITY;
+  t.bad = !(r.w == r.w) || r.m == INFINITY;
   t.empty = !t.bad && r.m == -INFINITY;
   const float nan = __int_as_float(0x7fffffff);
   t.m = t.bad ? nan : r.m;
   t.s = t.bad ? nan : t.empty ? 0.0f : r.s;
-  t.s1 = t.bad ? nan : t.empty ? 0.0f : r.s1;
-  t.log_s = t.bad ? (double)nan : t.empty ? (double)-INFINITY : log_det((double)r.s);
+  t.s1 = t.bad ? nan : t.empty ? 0.0f : fmul(r.w, kLn2);
   return t;
+}
+// log S in 64 bits
+DI double log_sum(const RowStats& r) {
+  return r.bad ? (double)__int_as_float(0x7fffffff) : r.empty ? (double)-INFINITY : log_det((double)r.s);
 }
 
 // order of the top list: larger values first, of equal values the lower
@@ -356,19 +501,23 @@ struct Teacher {
 
 // ---- the teacher's list of one row ---------------------------------------------
 struct ListShared {
-  float red[2][kThreads / 32];
-  int bad[kThreads / 32], some[kThreads / 32];
+  float max[kWarps], sum[kWarps];
+  int bad[kWarps], some[kWarps];
+  int id[DET_MAX_TOP];
+  float q[DET_MAX_TOP];
+  double term[kWarps];
 };
 struct ListEntry {
-  int id;       // -1: not a valid entry
-  float q;      // its share of the teacher's distribution
-  double logq;
+  int id;         // -1: not a valid entry
+  float q;        // its share of the teacher's distribution
+  float d;        // u - max u
+  bool some, bad;  // of the list: a valid entry; an id or value that is not allowed
+  float s;        // of the list: sum of exp(d / T)
 };
-// thread i < k of the block gets entry i (kThreads >= DET_MAX_TOP); *some: the
-// list has a valid entry; *bad: an id or value that is not allowed
-DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float temp, float one, ListShared& sh, bool* some,
-                           bool* bad) {
-  const int t = threadIdx.x, w = t >> 5, l = t & 31;
+// Thread i < k of the block gets entry i (blocks have at least DET_MAX_TOP
+// threads).  Begins and ends with the block in step.
+DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float c, float one, ListShared& sh) {
+  const int t = threadIdx.x, w = t >> 5, l = t & 31, nw = blockDim.x >> 5;
   long long id = -1;
   float u = -INFINITY;
   if (t < te.k) {
@@ -379,33 +528,69 @@ DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float temp, fl
   const bool valid = id >= 0 && !wrong && u > -INFINITY;
   float m = warp_max(valid ? u : -INFINITY);
   const int anyw = __any_sync(kFull, wrong), anyv = __any_sync(kFull, valid);
+  __syncthreads();
   if (l == 0) {
-    sh.red[0][w] = m;
+    sh.max[w] = m;
     sh.bad[w] = anyw;
     sh.some[w] = anyv;
   }
   __syncthreads();
   m = -INFINITY;
-  int b = 0, so = 0;
-  for (int i = 0; i < kThreads / 32; i++) {
-    m = fmaxf(m, sh.red[0][i]);
-    b |= sh.bad[i];
-    so |= sh.some[i];
-  }
-  const double du = valid ? ddiv(dsub((double)u, (double)m), (double)temp) : 0.0;
-  const float e = valid ? exp1(fmaxf((float)du, kExpLow), one) : 0.0f;
-  const float ws = warp_sum(e);
-  if (l == 0) sh.red[1][w] = ws;
-  __syncthreads();
-  float s = 0.0f;
-  for (int i = 0; i < kThreads / 32; i++) s = fadd(s, sh.red[1][i]);
-  *some = so != 0;
-  *bad = b != 0;
   ListEntry r;
+  r.some = r.bad = false;
+  for (int i = 0; i < nw; i++) {
+    m = fmaxf(m, sh.max[i]);
+    r.bad |= sh.bad[i] != 0;
+    r.some |= sh.some[i] != 0;
+  }
+  r.d = valid ? fsub(u, m) : 0.0f;
+  const float e = valid ? exp2_one(fmul(r.d, c), one) : 0.0f;
+  const float ws = warp_sum(e);
+  if (l == 0) sh.sum[w] = ws;
+  __syncthreads();
+  r.s = 0.0f;
+  for (int i = 0; i < nw; i++) r.s = fadd(r.s, sh.sum[i]);
   r.id = valid ? (int)id : -1;
-  r.q = valid ? fdiv(e, s) : 0.0f;
-  r.logq = valid ? dsub(du, log_det((double)s)) : 0.0;
+  r.q = valid ? fdiv(e, r.s) : 0.0f;
   return r;
+}
+// the row's loss, in thread 0; z: the logit at the thread's entry.  Ends with
+// the block in step.
+DI float list_loss(const ListEntry& e, float z, const RowStats& r, double log_s, float temp, ListShared& sh) {
+  double term = 0.0;
+  if (e.id >= 0 && e.q > 0.0f) {
+    const double logq = dsub(ddiv((double)e.d, (double)temp), log_det((double)e.s));
+    const double logp =
+        r.empty ? (double)-INFINITY : dsub(ddiv(dsub((double)z, (double)r.m), (double)temp), log_s);
+    term = dmul((double)e.q, dsub(logq, logp));
+  }
+  term = warp_sum_d(term);
+  if ((threadIdx.x & 31) == 0) sh.term[threadIdx.x >> 5] = term;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 5); i++) s = dadd(s, sh.term[i]);
+  const float nan = __int_as_float(0x7fffffff);
+  return e.bad ? nan : !e.some ? 0.0f : r.bad ? nan : (float)s;
+}
+// The share to take off at the thread's entry: what all entries of its id add
+// up to, in their order, at the first of them; 0 and id -1 at the others.
+DI float list_share(ListEntry& e, int k, ListShared& sh) {
+  __syncthreads();
+  if ((int)threadIdx.x < k) {
+    sh.id[threadIdx.x] = e.id;
+    sh.q[threadIdx.x] = e.q;
+  }
+  __syncthreads();
+  float sum = 0.0f;
+  if (e.id < 0) return sum;
+  bool first = true;
+  for (int i = 0; i < k; i++)
+    if (sh.id[i] == e.id) {
+      first &= i >= (int)threadIdx.x;
+      sum = fadd(sum, sh.q[i]);
+    }
+  if (!first) e.id = -1;
+  return sum;
 }
 
 // ---- the top list ------------------------------------------------------------------
@@ -419,23 +604,22 @@ constexpr int kCand = 2048;  // keys held before they are cut down to k
 struct TopShared {
   unsigned long long key[kCand + kThreads];
   int count, bits[2];
+  uint32_t lo, hi;
 };
 template <typename T>
 DI int group_size(int V) {
   return V <= kSmallVocab ? Seg<T>::VEC : Seg<T>::GROUP;
 }
-template <typename T>
-size_t groups_of(int V) {
-  const int g = V <= kSmallVocab ? Seg<T>::VEC : Seg<T>::GROUP, nseg = (V + kSeg - 1) / kSeg;
-  return (size_t)nseg * (kSeg / g);
-}
-
-// the largest t such that at least k of the block's values are >= t (0 where
-// there are fewer than k): bit by bit, done early once exactly k are
+// A t that at least k of the block's values reach, and at most k + slack of
+// them where values are not equal (0 where there are fewer than k): bit by
+// bit below the bits that all of [lo, hi] share; lo <= every value <= hi.
 template <typename K, int PER>
-DI K kth_largest(const K (&v)[PER], int k, TopShared& sh) {
-  K t = 0;
-  for (int bit = (int)sizeof(K) * 8 - 1, turn = 0; bit >= 0; bit--, turn ^= 1) {
+DI K kth_largest(const K (&v)[PER], K lo, K hi, int k, int slack, TopShared& sh) {
+  const K differ = lo ^ hi;
+  int bit = -1;
+  if (differ) bit = sizeof(K) == 8 ? 63 - __clzll((long long)differ) : 31 - __clz((int)differ);
+  K t = bit < 0 ? lo : lo & ~((K)2 * (((K)1 << bit) - 1) + 1);
+  for (int turn = 0; bit >= 0; bit--, turn ^= 1) {
     const K cand = t | ((K)1 << bit);
     int c = 0;
 #pragma unroll
@@ -447,7 +631,7 @@ DI K kth_largest(const K (&v)[PER], int k, TopShared& sh) {
     if (threadIdx.x == 0) sh.bits[turn ^ 1] = 0;
     __syncthreads();
     if (all >= k) t = cand;
-    if (all == k) break;
+    if (all >= k && all <= k + slack) break;
   }
   __syncthreads();
   if (threadIdx.x == 0) sh.bits[0] = sh.bits[1] = 0;
@@ -471,7 +655,7 @@ DI unsigned long long cut_to(int k, TopShared& sh) {
     const int at = i * kThreads + threadIdx.x;
     v[i] = at < n ? sh.key[at] : 0;
   }
-  const unsigned long long t = kth_largest<unsigned long long, PER>(v, k, sh);
+  const unsigned long long t = kth_largest<unsigned long long, PER>(v, 0ull, ~0ull, k, 0, sh);
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
 #pragma unroll
@@ -515,25 +699,39 @@ DI void collect(const T* __restrict__ x, int V, int mis, const float* gmax, int 
     }
   }
 }
+template <int PER>
+DI unsigned long long list_floor(const float* gmax, int ng, int k, TopShared& sh) {
+  uint32_t v[PER], lo = ~0u, hi = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int g = i * kThreads + threadIdx.x;
+    const bool is = g < ng;
+    v[i] = is ? (uint32_t)(top_key(gmax[g], 0) >> 32) : 0u;
+    hi = max(hi, v[i]);
+    if (is) lo = min(lo, v[i]);
+  }
+  hi = __reduce_max_sync(kFull, hi);
+  lo = __reduce_min_sync(kFull, lo);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMax(&sh.hi, hi);
+    atomicMin(&sh.lo, lo);
+  }
+  __syncthreads();
+  const uint32_t t = kth_largest<uint32_t, PER>(v, sh.lo, sh.hi, k, k / 4 + 4, sh);
+  return t ? ((unsigned long long)t << 32) - 1 : 0;
+}
 // the row's k largest keys, in order, to sh.key[0 .. k)
 template <typename T>
 DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int k, TopShared& sh) {
   const int ng = (V + group_size<T>(V) - 1) / group_size<T>(V);
-  if (threadIdx.x == 0) sh.count = sh.bits[0] = sh.bits[1] = 0;
+  if (threadIdx.x == 0) sh.count = sh.bits[0] = sh.bits[1] = 0, sh.lo = ~0u, sh.hi = 0;
   __syncthreads();
-  // a value that at least k entries reach: the k-th largest maximum
+  // a value that at least k entries reach: about the k-th largest maximum
   unsigned long long floor = 0;
   if (ng > k) {
-    constexpr int PER = kSmallVocab / Seg<T>::VEC / kThreads;  // as many groups as there can be, or more
-    static_assert(PER * kThreads >= (int)kMaxVocab / Seg<T>::GROUP, "every group has a place");
-    uint32_t v[PER];
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int g = i * kThreads + threadIdx.x;
-      v[i] = g < ng ? (uint32_t)(top_key(gmax[g], 0) >> 32) : 0u;
-    }
-    const uint32_t t = kth_largest<uint32_t, PER>(v, k, sh);
-    floor = t ? ((unsigned long long)t << 32) - 1 : 0;
+    floor = ng <= kThreads * 4   ? list_floor<4>(gmax, ng, k, sh)
+            : ng <= kThreads * 8 ? list_floor<8>(gmax, ng, k, sh)
+                                 : list_floor<kSmallVocab / 4 / kThreads>(gmax, ng, k, sh);
   }
   collect<T>(x, V, mis, gmax, 0, ng, floor, sh);
   __syncthreads();
@@ -585,126 +783,130 @@ DI uint32_t remote(const void* p, uint32_t rank) {
 }
 DI void store_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 
+// what a row's scores are written to (one thread)
+DI void write_stats(float* stats, int row, const RowStats& r, double log_s) {
+  float* st = stats + (size_t)row * 4;
+  st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = (float)log_s;
+}
+DI void write_scores(const ScoreOut& o, int row, int V, const RowStats& r, double log_s, long long t, float x_t) {
+  const float nan = __int_as_float(0x7fffffff);
+  if (o.entropy)
+    o.entropy[row] = r.bad ? nan : r.empty ? 0.0f : (float)dsub(log_s, ddiv((double)r.s1, (double)r.s));
+  if (!o.logprob) return;
+  float v;
+  if (r.bad || t >= V) v = nan;
+  else if (t < 0) v = 0.0f;
+  else if (r.empty) v = -INFINITY;
+  else v = (float)dsub(dsub((double)x_t, (double)r.m), log_s);
+  o.logprob[row] = v;
+}
+
 // ---- forward ---------------------------------------------------------------------------
-// One cluster per row (of one block where there are rows enough): its warps
-// take segments in turn, their sums and group maxima go to block 0, which
-// joins them and writes the row's results.
-struct ForwardShared {
-  float m[kMaxSegs], s[kMaxSegs], w[kMaxSegs];
-  RowStats row;
-  ListShared list;
-  double dred[kThreads / 32];
+constexpr int kSegThreads = 256, kSegBlocks = 2;
+// Two kernels.  In the first, warps take segments in turn, whatever row they
+// are of, each with its next one on its way; nothing waits for anything else,
+// and the parts are even however many rows there are.  A segment's sums and
+// its groups' maxima go to the caller's workspace.  In the second, a block per
+// row joins the row's segments and writes its results.
+struct Workspace {
+  float4* seg;  // [rows][segments]: m, s, w
+  float* gmax;  // [rows][groups]
 };
-template <typename T, bool TOP, bool SCALED>
-__global__ void __launch_bounds__(kThreads, 2)
-    forward_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, float* loss, ScoreOut o,
-                   float one) {
+enum : int { GROUPS_NONE, GROUPS_LANE, GROUPS_WARP };  // which maxima a top list needs
+template <typename T, int GROUPS>
+__global__ void __launch_bounds__(kSegThreads, kSegBlocks)
+    segments_kernel(Logits L, float temp, Workspace ws, float one) {
   using G = Seg<T>;
-  __shared__ ForwardShared sh;
-  extern __shared__ float dyn[];  // TOP: group maxima, then a TopShared
-  const uint32_t rank = cluster_rank(), size = cluster_size();
-  const int row = blockIdx.x / size, V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
-  const int nseg = (V + kSeg - 1) / kSeg, mis = misaligned(x);
-  const float inv_t = SCALED ? fdiv(1.0f, temp) : 1.0f;
-  if (size > 1) cluster_arrive();  // block 0 runs before anyone writes to it
-  bool first = size > 1;
-  for (int g = rank * (kThreads / 32) + w; g < nseg; g += size * (kThreads / 32)) {
-    float v[kPerLane];
-    load_segment<T>(x, g, V, mis, v);
-    float m = -INFINITY, gm = -INFINITY;
-    float lm[G::NV];
+  extern __shared__ __align__(16) uint8_t dyn[];  // a stage per warp
+  const int V = L.vocab, l = threadIdx.x & 31;
+  const int nseg = (V + kSeg - 1) / kSeg, all = gridDim.x * (kSegThreads / 32);
+  void* stage = dyn + (threadIdx.x >> 5) * kStageBytes<T>;
+  auto at_row = [&](int r) { return static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[r] : r) * L.ld; };
+  const int first = blockIdx.x * (kSegThreads / 32) + (threadIdx.x >> 5);
+  int row = first / nseg, g = first % nseg;
+  const int drow = all / nseg, dg = all % nseg;
+  if (row < L.n) stage_issue<T>(stage, at_row(row), g, V);
+  pdl_trigger();
+  const float c = fdiv(kLog2e, temp);
+  const uint32_t table = kExpTable[l];
+  while (row < L.n) {
+    uint4 v[G::NV];
+    stage_take<T>(stage, misaligned(at_row(row)), v);
+    int nrow = row + drow, ng = g + dg;
+    if (ng >= nseg) ng -= nseg, nrow++;
+    if (nrow < L.n) stage_issue<T>(stage, at_row(nrow), ng, V);
+    float m = -INFINITY, low = INFINITY, gm = -INFINITY;
+    const size_t part = (size_t)row * nseg + g;
+    float* gmax = ws.gmax + part * (kSeg / G::VEC) + l;
 #pragma unroll
     for (int i = 0; i < G::NV; i++) {
-      lm[i] = v[i * G::VEC];
-#pragma unroll
-      for (int j = 1; j < G::VEC; j++) lm[i] = fmaxf(lm[i], v[i * G::VEC + j]);
-      m = fmaxf(m, lm[i]);
-      if constexpr (TOP) {
-        const float r = redux_max(lm[i]);
+      float lm, ll;
+      vec_range<T>(v[i], lm, ll);
+      m = fmaxf(m, lm);
+      low = fminf(low, ll);
+      if constexpr (GROUPS == GROUPS_LANE) gmax[i * 32] = lm;
+      if constexpr (GROUPS == GROUPS_WARP) {
+        const float r = redux_max(lm);
         if (l == i) gm = r;
       }
     }
+    if constexpr (GROUPS == GROUPS_WARP) {
+      if (l < G::NV) ws.gmax[part * G::NV + l] = gm;
+    }
     m = redux_max(m);
-    const Sums r = segment_sums<SCALED>(v, m, inv_t, one);
-    if (first) cluster_wait();
-    first = false;
-    if (l == 0) {
-      store_remote(remote(&sh.m[g], 0), r.m);
-      store_remote(remote(&sh.s[g], 0), r.s);
-      store_remote(remote(&sh.w[g], 0), r.s1);
-    }
-    if constexpr (TOP) {
-      if (V <= kSmallVocab) {
-#pragma unroll
-        for (int i = 0; i < G::NV; i++) store_remote(remote(&dyn[g * (kSeg / G::VEC) + i * 32 + l], 0), lm[i]);
-      } else if (l < G::NV) {
-        store_remote(remote(&dyn[g * G::NV + l], 0), gm);
-      }
-    }
+    low = redux_min(low);
+    const float s = segment_sums<T, false>(v, V - g * kSeg, m, low, c, table, one, nullptr);
+    const float w = __shfl_sync(kFull, s, 16);
+    if (l == 0) ws.seg[part] = make_float4(m, s, w, 0.0f);
+    row = nrow;
+    g = ng;
   }
-  if (size > 1) {
-    if (first) cluster_wait();
-    cluster_arrive();
-    cluster_wait();
-    if (rank != 0) return;
-  } else {
-    __syncthreads();
-  }
-  if (w == 0) {
-    const RowStats r = finish_row(join_segments(sh.m, sh.s, sh.w, nseg, inv_t, one));
-    if (l == 0) {
-      sh.row = r;
-      if (o.stats) {
-        float* st = o.stats + (size_t)row * 4;
-        st[0] = r.m, st[1] = r.s, st[2] = r.s1, st[3] = (float)r.log_s;
-      }
-      if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
-    }
-  }
-  __syncthreads();
-  const RowStats r = sh.row;
-  const float nan = __int_as_float(0x7fffffff);
+}
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(TOP ? kThreads : (int)DET_MAX_TOP)
+    rows_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, Workspace ws, float* loss,
+                ScoreOut o, float one) {
+  __shared__ ListShared list;
+  const int row = blockIdx.x, V = L.vocab, nseg = (V + kSeg - 1) / kSeg;
+  const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
+  const float c = fdiv(kLog2e, temp), nan = __int_as_float(0x7fffffff);
+  // what does not depend on the sums, while they are being taken
+  ListEntry e;
+  float z = 0.0f;
+  long long t = -1;
   if (loss) {
-    bool some, bad;
-    const ListEntry e = teacher_entry(te, row, V, temp, one, sh.list, &some, &bad);
-    double term = 0.0;
-    if (e.id >= 0 && e.q > 0.0f) {
-      const double z = (double)to_f32(x[e.id]);
-      const double logp = r.empty ? (double)-INFINITY : dsub(ddiv(dsub(z, (double)r.m), (double)temp), r.log_s);
-      term = dmul((double)e.q, dsub(e.logq, logp));
-    }
-    term = warp_sum_d(term);
-    if (l == 0) sh.dred[w] = term;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double s = 0.0;
-      for (int i = 0; i < kThreads / 32; i++) s = dadd(s, sh.dred[i]);
-      loss[row] = bad ? nan : !some ? 0.0f : r.bad ? nan : (float)s;
-      if (bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
-    }
-    return;
+    e = teacher_entry(te, row, V, c, one, list);
+    if (e.id >= 0) z = to_f32(x[e.id]);
+  } else if (o.logprob) {
+    t = load_id(tokens, id_bytes, row);
+    if (t >= 0 && t < V) z = to_f32(x[t]);
   }
+  pdl_wait();
+  const float4* seg = ws.seg + (size_t)row * nseg;
+  const RowStats r = finish_row(join_segments(
+      [&](int i) {
+        const float4 f = seg[i];
+        return Sums{f.x, f.y, f.z};
+      },
+      nseg, c, one));
+  const double log_s = log_sum(r);
   if (threadIdx.x == 0) {
-    if (o.entropy) {
-      o.entropy[row] = r.bad     ? nan
-                       : r.empty ? 0.0f
-                                 : (float)dsub(r.log_s, ddiv((double)r.s1, (double)r.s));
+    if (o.stats) write_stats(o.stats, row, r, log_s);
+    if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+  }
+  if (loss) {
+    const float v = list_loss(e, z, r, log_s, temp, list);
+    if (threadIdx.x == 0) {
+      loss[row] = v;
+      if (e.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
     }
-    if (o.logprob) {
-      const long long t = load_id(tokens, id_bytes, row);
-      float v;
-      if (r.bad || t >= V) v = nan;
-      else if (t < 0) v = 0.0f;
-      else if (r.empty) v = -INFINITY;
-      else v = (float)dsub(dsub((double)to_f32(x[t]), (double)r.m), r.log_s);
-      o.logprob[row] = v;
-      if (t >= V && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
-    }
+  } else if (threadIdx.x == 0) {
+    write_scores(o, row, V, r, log_s, t, z);
+    if (t >= V && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
   }
   if constexpr (TOP) {
-    TopShared& top = *reinterpret_cast<TopShared*>(dyn + (size_t)nseg * (kSeg / group_size<T>(V)));
-    if (!r.bad) top_list<T>(x, V, mis, dyn, o.top, top);
+    __shared__ TopShared top;
+    if (!r.bad) top_list<T>(x, V, misaligned(x), ws.gmax + (size_t)row * nseg * (kSeg / group_size<T>(V)), o.top, top);
     if ((int)threadIdx.x < o.top) {
       const size_t at = (size_t)row * o.top + threadIdx.x;
       const unsigned long long key = r.bad ? 0 : top.key[threadIdx.x];
@@ -712,179 +914,396 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (o.top_logprobs) {
         o.top_logprobs[at] = r.bad     ? nan
                              : r.empty ? -INFINITY
-                                       : (float)dsub(dsub((double)key_value(key), (double)r.m), r.log_s);
+                                       : (float)dsub(dsub((double)key_value(key), (double)r.m), log_s);
       }
     }
   }
 }
 
 // ---- gradient --------------------------------------------------------------------------
-// dx_j = exp(d_j) (a + b d_j) + (what the row's own tokens add).  `as`, `bs`
-// are a and b over S.
+// dx_j = 2^y_j (a + b y_j) / S + (what the row's own tokens add), y = (x - m)
+// log2(e) / T; b is 0 but for the entropy's gradient.
 struct GradIn {
   const float *stats, *g, *gh;  // g: of logprob or of the loss; gh: of the entropy, or null
 };
 struct RowGrad {
-  float base, inv_t, as, bs;  // base: -m
-  bool zero;                  // nothing but zeros
+  float base, c, as, bs;  // -m, log2(e) / T, a / S, b / S
+  bool zero;              // nothing but zeros
 };
-struct GradShared {
-  ListShared list;
-  int id[DET_MAX_TOP];
-  float add[DET_MAX_TOP];
-};
-// gradients of a pair of entries
-template <bool ENTROPY, bool SCALED>
-DI f2 grad2(f2 x, const RowGrad& r, f2 one) {
-  f2 d = add2(x, pk(r.base, r.base));
-  if constexpr (SCALED) d = mul2(d, pk(r.inv_t, r.inv_t));
-  const Exp2 e = exp2_lanes(d, one);
-  if constexpr (ENTROPY) return mul2(e.e, addp(mul2(e.d, pk(r.bs, r.bs)), one, pk(r.as, r.as)));
-  return mul2(e.e, pk(r.as, r.as));
-}
-// the row's coefficients, and in sh what its tokens add: id[i] (or -1) and
-// add[i] for i < the returned count.  Ends with a barrier.
-DI int row_grad(int row, int V, const void* tokens, int id_bytes, const Teacher& te, float temp, const GradIn& in,
-                float m, float s, float s1, float one, GradShared& sh, RowGrad& r) {
-  const float nan = __int_as_float(0x7fffffff);
+// the coefficients of a row of scores; gl: what its token adds
+DI RowGrad score_grad(const GradIn& in, int row, int V, long long t, float m, float s, float s1, float c, float* gl) {
   const bool empty = m == -INFINITY;
-  const float g = in.g ? in.g[row] : 0.0f;
-  float a, b = 0.0f;
-  bool blank = false;
-  int k = 1;
-  if (te.k) {
-    bool some, bad;
-    const ListEntry e = teacher_entry(te, row, V, temp, one, sh.list, &some, &bad);
-    blank = !some && !bad;
-    a = bad ? nan : fdiv(g, temp);
-    k = te.k;
-    if ((int)threadIdx.x < k) {
-      sh.id[threadIdx.x] = e.id;
-      sh.add[threadIdx.x] = e.q;
-    }
-    __syncthreads();
-    // an id that is listed twice: its first entry takes the sum, in order
-    float sum = 0.0f;
-    bool first = true;
-    if ((int)threadIdx.x < k && e.id >= 0)
-      for (int i = 0; i < k; i++)
-        if (sh.id[i] == e.id) {
-          if (i < (int)threadIdx.x) first = false;
-          sum = fadd(sum, sh.add[i]);
-        }
-    __syncthreads();
-    if ((int)threadIdx.x < k) {
-      if (!first) sh.id[threadIdx.x] = -1;
-      sh.add[threadIdx.x] = fmul(-a, sum);
-    }
-  } else {
-    const float gh = in.gh ? in.gh[row] : 0.0f;
-    const long long t = in.g ? load_id(tokens, id_bytes, row) : -1;
-    const float gl = t < 0 ? 0.0f : t >= V ? nan : g;
-    a = fadd(-gl, fmul(gh, fdiv(s1, s)));
-    b = -gh;
-    if (threadIdx.x == 0) {
-      sh.id[0] = t >= 0 && t < V ? (int)t : -1;
-      sh.add[0] = gl;
-    }
-  }
+  const float gh = in.gh ? in.gh[row] : 0.0f;
+  *gl = !in.g || t < 0 ? 0.0f : t >= V ? __int_as_float(0x7fffffff) : in.g[row];
   const float inv_s = fdiv(1.0f, s);
-  r.zero = blank || empty;
-  r.base = -m;
-  r.inv_t = fdiv(1.0f, temp);
-  r.as = fmul(a, inv_s);
-  r.bs = fmul(b, inv_s);
-  __syncthreads();
-  return k;
+  return {-m, c, fmul(fadd(-*gl, fmul(gh, fdiv(s1, s))), inv_s), fmul(fmul(-gh, kLn2), inv_s), empty};
+}
+// and of a row against a list; g_t: gradient of the loss over T
+DI RowGrad list_grad(const ListEntry& e, float g_t, float m, float s, float c) {
+  const float a = e.bad ? __int_as_float(0x7fffffff) : g_t;
+  return {-m, c, fmul(a, fdiv(1.0f, s)), 0.0f, (!e.some && !e.bad) || m == -INFINITY};
+}
+// gradients of a pair of entries (of one, with the same bits)
+template <bool ENTROPY>
+DI f2 grad2(f2 e, f2 y, const RowGrad& r, f2 one) {
+  if constexpr (ENTROPY) return mul2(e, addp(mul2(y, pk(r.bs, r.bs)), one, pk(r.as, r.as)));
+  return mul2(e, pk(r.as, r.as));
+}
+template <bool ENTROPY>
+DI float grad1(float x, const RowGrad& r, float one) {
+  const float y = max_nan(fmul(fadd(x, r.base), r.c), kYLow);
+  return un(grad2<ENTROPY>(pk(exp2_one(y, one), 0.0f), pk(y, 0.0f), r, pk(one, one))).x;
 }
 
 // Blocks (blockIdx.x) of a row (blockIdx.y + row0) take `per` of its 16-byte
 // vectors each; a vector is one of the gradient's, so that stores are whole
-// wherever the row starts.  `out` may be the logits themselves.
+// wherever the row starts.  The next vectors are loaded before these are
+// worked on, the first ones before the row's coefficients are known.  `out`
+// may be the logits themselves.
 constexpr int kGradUnroll = 4;
-template <typename T, bool ENTROPY, bool SCALED>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kThreads, 3)
     grad_kernel(Logits L, int row0, int per, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in,
                 T* out, unsigned long long out_ld, float one_) {
-  constexpr int VEC = Seg<T>::VEC;
-  __shared__ GradShared sh;
+  constexpr int VEC = Seg<T>::VEC, U = kGradUnroll;
+  __shared__ ListShared sh;
   const int row = row0 + blockIdx.y, V = L.vocab;
   const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
   T* y = out + (size_t)row * out_ld;
-  const float* st = in.stats + (size_t)row * 4;
-  RowGrad r;
-  const int k = row_grad(row, V, tokens, id_bytes, te, temp, in, st[0], st[1], st[2], one_, sh, r);
-  const f2 one = pk(one_, one_);
   const int my = misaligned(y), mis = (misaligned(x) - my) & (VEC - 1);
   const int nvec = (V + my + VEC - 1) / VEC;
   const int q0 = blockIdx.x * per, q1 = min(nvec, q0 + per);
+  auto whole = [&](int at) { return at >= 0 && at + VEC <= V; };
+  auto fetch = [&](int q, uint4(&w)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = (q + u * kThreads) * VEC - my;
+      if (q + u * kThreads >= q1 || !whole(at)) continue;
+      const T* p = x + at;
+      if (mis == 0) {
+        w[u] = *reinterpret_cast<const uint4*>(p);
+      } else if (at >= mis && at - mis + 2 * VEC <= V) {
+        const uint4* g = reinterpret_cast<const uint4*>(p - mis);
+        w[u] = shifted(g[0], g[1], mis * (int)sizeof(T));
+      } else {
+        float v[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = to_f32(p[j]);
+        w[u] = pack_vec<T>(v);
+      }
+    }
+  };
+  uint4 cur[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) cur[u] = make_uint4(0, 0, 0, 0);
+  fetch(q0 + threadIdx.x, cur);
+  const float* st = in.stats + (size_t)row * 4;
+  const float m = st[0], s = st[1], c = fdiv(kLog2e, temp);
+  const uint32_t table = kExpTable[threadIdx.x & 31];
+  RowGrad r;
+  int id;
+  float add;
+  if (te.k) {
+    ListEntry e = teacher_entry(te, row, V, c, one_, sh);
+    const float g_t = fdiv(in.g[row], temp);
+    r = list_grad(e, g_t, m, s, c);
+    add = fmul(-g_t, list_share(e, te.k, sh));
+    id = e.id;
+  } else {
+    const long long t = in.g ? load_id(tokens, id_bytes, row) : -1;
+    r = score_grad(in, row, V, t, m, s, st[2], c, &add);
+    id = threadIdx.x == 0 && t >= 0 && t < V ? (int)t : -1;
+  }
   // the values at the row's own tokens, before `out` may overwrite them
-  const int id = (int)threadIdx.x < k ? sh.id[threadIdx.x] : -1;
   const bool patch = id >= 0 && id >= q0 * VEC - my && id < q1 * VEC - my && !r.zero;
   float mine = 0.0f;
-  if (patch) {
-    const float v = to_f32(x[id]);
-    mine = fadd(un(grad2<ENTROPY, SCALED>(pk(v, v), r, one)).x, sh.add[threadIdx.x]);
-  }
+  if (patch) mine = fadd(grad1<ENTROPY>(to_f32(x[id]), r, one_), add);
   __syncthreads();
-  for (int q = q0 + threadIdx.x; q < q1; q += kThreads * kGradUnroll) {
-    float v[kGradUnroll][VEC];
+  const f2 one = pk(one_, one_), base = pk(r.base, r.base), cc = pk(c, c);
+  for (int b = q0; b < q1; b += kThreads * U) {  // the same turns for all lanes: exp2_warp shuffles
+    const int q = b + threadIdx.x;
+    uint4 next[U];
 #pragma unroll
-    for (int u = 0; u < kGradUnroll; u++) {
-      const int at = (q + u * kThreads) * VEC - my;
-      if (q + u * kThreads < q1) load_vec<T, false>(x, at, V, mis, v[u]);
+    for (int u = 0; u < U; u++) next[u] = make_uint4(0, 0, 0, 0);
+    fetch(q + kThreads * U, next);
+    // no entry of the warp is so far below the maximum that it has to be
+    // cleared (vectors that are not whole are left out: not safe)
+    float low = INFINITY, high;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float lo;
+      vec_range<T>(cur[u], high, lo);
+      const bool in_row = q + u * kThreads < q1;
+      low = fminf(low, !in_row ? INFINITY : whole((q + u * kThreads) * VEC - my) ? lo : -INFINITY);
     }
+    const bool safe = fmul(fadd(redux_min(low), r.base), c) >= kYSafe;
 #pragma unroll
-    for (int u = 0; u < kGradUnroll; u++) {
+    for (int u = 0; u < U; u++) {
       const int at = (q + u * kThreads) * VEC - my;
-      if (q + u * kThreads >= q1) continue;
+      const bool in_row = q + u * kThreads < q1;
+      float v[VEC];
+      unpack_vec<T>(cur[u], v);
+      if (in_row && !whole(at)) {
 #pragma unroll
-      for (int j = 0; j < VEC; j += 2) {
-        const float2 gr = un(grad2<ENTROPY, SCALED>(pk(v[u][j], v[u][j + 1]), r, one));
-        v[u][j] = r.zero ? 0.0f : gr.x;
-        v[u][j + 1] = r.zero ? 0.0f : gr.y;
+        for (int j = 0; j < VEC; j++) v[j] = at + j >= 0 && at + j < V ? to_f32(x[at + j]) : 0.0f;
       }
-      if (at >= 0 && at + VEC <= V) {
-        *reinterpret_cast<uint4*>(y + at) = pack_vec<T>(v[u]);
+      if (safe) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const Exp2 e = exp2_warp<false>(mul2(add2(pk(v[j], v[j + 1]), base), cc), table, one);
+          const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
+          v[j] = gr.x;
+          v[j + 1] = gr.y;
+        }
       } else {
 #pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const Exp2 e = exp2_warp<true>(mul2(add2(pk(v[j], v[j + 1]), base), cc), table, one);
+          const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
+          v[j] = gr.x;
+          v[j + 1] = gr.y;
+        }
+      }
+      if (r.zero) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = 0.0f;
+      }
+      if (in_row && whole(at)) {
+        *reinterpret_cast<uint4*>(y + at) = pack_vec<T>(v);
+      } else if (in_row) {
+#pragma unroll
         for (int j = 0; j < VEC; j++)
-          if (at + j >= 0 && at + j < V) y[at + j] = from_f32<T>(v[u][j]);
+          if (at + j >= 0 && at + j < V) y[at + j] = from_f32<T>(v[j]);
       }
     }
+#pragma unroll
+    for (int u = 0; u < U; u++) cur[u] = next[u];
   }
   __syncthreads();
   if (patch) y[id] = from_f32<T>(mine);
+}
+
+// ---- both at once ------------------------------------------------------------------------
+// Stores a warp's segment: vectors where the row is aligned; elsewhere lane l
+// puts together the granule its vector starts in from its neighbour's end and
+// its own start.
+template <typename T, typename F>
+DI void store_segment(T* y, int g, int V, int my, F vec) {
+  using G = Seg<T>;
+  constexpr int VEC = G::VEC;
+  const int l = threadIdx.x & 31, lo = g * kSeg, hi = min(V, lo + kSeg);
+  auto put = [&](int at, uint4 w) {  // what of [at, at + VEC) is in [lo, hi)
+    if (at >= lo && at + VEC <= hi) {
+      *reinterpret_cast<uint4*>(y + at) = w;
+    } else {
+      float f[VEC];
+      unpack_vec<T>(w, f);
+#pragma unroll
+      for (int j = 0; j < VEC; j++)
+        if (at + j >= lo && at + j < hi) y[at + j] = from_f32<T>(f[j]);
+    }
+  };
+  if (my == 0) {
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) put(lo + (32 * i + l) * VEC, vec(i));
+    return;
+  }
+  uint4 carry = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < G::NV; i++) {
+    const uint4 w = vec(i);
+    uint4 p;  // of the lane before; lane 0 gets lane 31's, for the next turn
+    p.x = __shfl_sync(kFull, w.x, (l + 31) & 31);
+    p.y = __shfl_sync(kFull, w.y, (l + 31) & 31);
+    p.z = __shfl_sync(kFull, w.z, (l + 31) & 31);
+    p.w = __shfl_sync(kFull, w.w, (l + 31) & 31);
+    const uint4 before = l == 0 ? carry : p;
+    carry = p;
+    put(lo + (32 * i + l) * VEC - my, shifted(before, w, 16 - my * (int)sizeof(T)));
+    if (i == G::NV - 1 && l == 31) put(lo + kSeg - my, shifted(w, w, 16 - my * (int)sizeof(T)));
+  }
+}
+
+// Clusters take rows in turn; each of a cluster's warps holds one segment of
+// the row, so the row is read once: its exponentials stay in registers until
+// every block has all segments' sums, and are scaled and stored then, while
+// the next row's segment is on its way.  The entropy's gradient needs y too:
+// it keeps the logits and takes their exponentials again.
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kThreads, 2)
+    step_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, float* loss,
+                ScoreOut o, T* out, unsigned long long out_ld, float one_) {
+  __shared__ struct {
+    float m[kMaxSegs], s[kMaxSegs], w[kMaxSegs];
+    ListShared list;
+  } sh;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const int V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int nseg = (V + kSeg - 1) / kSeg, clusters = gridDim.x / size;
+  const int g = rank * warps + w;
+  const bool active = g < nseg;
+  void* stage = dyn + w * kStageBytes<T>;
+  auto at_row = [&](int r) { return static_cast<const T*>(L.x) + (size_t)r * L.ld; };
+  int row = blockIdx.x / size;
+  if (row < L.n && active) stage_issue<T>(stage, at_row(row), g, V);
+  const float c = fdiv(kLog2e, temp);
+  const uint32_t table = kExpTable[l];
+  if (size > 1) cluster_arrive();
+  for (; row < L.n; row += clusters) {
+    const T* x = at_row(row);
+    T* y = out + (size_t)row * out_ld;
+    uint4 raw[Seg<T>::NV];
+    float v[ENTROPY ? 1 : kPerLane];
+    float m_seg = -INFINITY, s_seg = 0.0f, w_seg = 0.0f;
+    if (active) {
+      stage_take<T>(stage, misaligned(x), raw);
+      if (row + clusters < L.n) stage_issue<T>(stage, at_row(row + clusters), g, V);
+      float low = INFINITY;
+#pragma unroll
+      for (int i = 0; i < Seg<T>::NV; i++) {
+        float h, l;
+        vec_range<T>(raw[i], h, l);
+        m_seg = fmaxf(m_seg, h);
+        low = fminf(low, l);
+      }
+      m_seg = redux_max(m_seg);
+      s_seg = segment_sums<T, !ENTROPY>(raw, V - g * kSeg, m_seg, redux_min(low), c, table, one_, v);
+      w_seg = __shfl_sync(kFull, s_seg, 16);
+      s_seg = __shfl_sync(kFull, s_seg, 0);
+    }
+    // the row's own tokens, before `out` may overwrite their logits
+    ListEntry e;
+    long long t = -1;
+    int id;
+    float share = 0.0f;
+    if (te.k) {
+      e = teacher_entry(te, row, V, c, one_, sh.list);
+      id = e.id;
+    } else {
+      t = tokens ? load_id(tokens, id_bytes, row) : -1;
+      id = threadIdx.x == 0 && t >= 0 && t < V ? (int)t : -1;
+    }
+    const float z = id >= 0 ? to_f32(x[id]) : 0.0f;
+    if (te.k) {
+      ListEntry f = e;
+      share = list_share(f, te.k, sh.list);
+      id = f.id;
+    }
+    if (size > 1) cluster_wait();
+    else __syncthreads();
+    if (active && l < (int)size) {
+      store_remote(remote(&sh.m[g], l), m_seg);
+      store_remote(remote(&sh.s[g], l), s_seg);
+      store_remote(remote(&sh.w[g], l), w_seg);
+    }
+    if (size > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+    const RowStats r =
+        finish_row(join_segments([&](int i) { return Sums{sh.m[i], sh.s[i], sh.w[i]}; }, nseg, c, one_));
+    if (size > 1) cluster_arrive();
+    RowGrad rg;
+    float add;
+    if (te.k) {
+      const float g_t = fdiv(in.g[row], temp);
+      rg = list_grad(e, g_t, r.m, r.s, c);
+      add = fmul(-g_t, share);
+    } else {
+      rg = score_grad(in, row, V, t, r.m, r.s, r.s1, c, &add);
+    }
+    if (active) {
+      const f2 one = pk(one_, one_), base = pk(rg.base, rg.base), cc = pk(c, c);
+      const float f = fmul(exp2_one(segment_y(m_seg, r.m, c), one_), rg.as);
+      // vector i of the segment's gradient
+      auto vec = [&](int i) {
+        constexpr int VEC = Seg<T>::VEC;
+        float x[VEC];
+        if constexpr (ENTROPY) unpack_vec<T>(raw[i], x);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          f2 d;
+          if constexpr (ENTROPY) {
+            const Exp2 ex = exp2_warp<true>(mul2(add2(pk(x[j], x[j + 1]), base), cc), table, one);
+            d = grad2<true>(ex.e, ex.y, rg, one);
+          } else {
+            d = mul2(pk(v[i * VEC + j], v[i * VEC + j + 1]), pk(f, f));
+          }
+          const float2 dv = un(d);
+          x[j] = rg.zero ? 0.0f : dv.x;
+          x[j + 1] = rg.zero ? 0.0f : dv.y;
+        }
+        return pack_vec<T>(x);
+      };
+      store_segment<T>(y, g, V, misaligned(y), vec);
+    }
+    if (rank == 0) {
+      const double log_s = log_sum(r);
+      if (threadIdx.x == 0) {
+        if (o.stats) write_stats(o.stats, row, r, log_s);
+        if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+        if ((te.k ? e.bad : t >= V) && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
+        if (!te.k) write_scores(o, row, V, r, log_s, t, z);
+      }
+      if (te.k) {
+        const float lv = list_loss(e, z, r, log_s, temp, sh.list);
+        if (threadIdx.x == 0) loss[row] = lv;
+      }
+    }
+    __syncthreads();  // the segments are stored
+    if (id >= (int)rank * warps * kSeg && id < (int)(rank + 1) * warps * kSeg && !rg.zero)
+      y[id] = from_f32<T>(fadd(grad1<ENTROPY>(z, rg, one_), add));
+  }
+  if (size > 1) cluster_wait();
 }
 
 // ---- launches --------------------------------------------------------------------
 template <typename F>
 cudaError_t by_dtype(int dtype, F f) {
   switch (dtype) {
-    case DET_DTYPE_F32: f(float{}); break;
-    case DET_DTYPE_F16: f(__half{}); break;
-    default: f(__nv_bfloat16{}); break;
+    case DET_DTYPE_F32: return f(float{});
+    case DET_DTYPE_F16: return f(__half{});
+    default: return f(__nv_bfloat16{});
   }
-  return cudaGetLastError();
 }
 
-// Blocks per row: enough for the GPU (two blocks of 8 warps per SM) while
-// every warp keeps a segment.
-int cluster_for(int n, int vocab) {
-  const int nseg = (vocab + kSeg - 1) / kSeg, sms = device_sms();
-  int c = 1;
-  while (c < 8 && (long long)n * c < 2 * sms && nseg > c * (kThreads / 32)) c *= 2;
-  return c;
-}
-template <typename T, bool TOP, bool SCALED>
-cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te,
-                       float temp, float* loss, const ScoreOut& o) {
-  const size_t smem = TOP ? groups_of<T>(L.vocab) * sizeof(float) + sizeof(TopShared) : 0;
-  if (cudaError_t e = raise_smem_cap((const void*)forward_kernel<T, TOP, SCALED>, smem)) return e;
-  const int c = cluster_for(L.n, L.vocab);
+// Clusters of `c` blocks that the current device holds at once, at least 1
+// (cached: the answer depends on the kernel and the launch alone).
+int resident_clusters(const void* kern, int c, int threads, size_t smem) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int, int, size_t>, int> known;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[{kern, dev, c, threads, smem}];
+  if (n > 0) return n;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(L.n * c));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)c);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int got = 0;
+  if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess || got < 1) {
+    cudaGetLastError();
+    got = 1;
+  }
+  return n = got;
+}
+// launches `clusters` clusters of c blocks
+template <typename... KArgs, typename... Args>
+cudaError_t launch_clusters(cudaStream_t s, void (*kern)(KArgs...), int clusters, int c, int threads, size_t smem,
+                            Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * c));
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -893,30 +1312,68 @@ cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = c > 1;
-  return cudaLaunchKernelEx(&cfg, forward_kernel<T, TOP, SCALED>, L, tokens, id_bytes, te, temp, loss, o, 1.0f);
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+// clusters above 8 blocks have to be allowed, once per kernel and device
+cudaError_t allow_large_clusters(const void* kern) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kern, dev})) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.insert({kern, dev});
+  return e;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+// what a forward call keeps between its two kernels
+size_t workspace_bytes(int dtype, int n, int vocab, int top) {
+  const size_t nseg = (vocab + kSeg - 1) / kSeg, vec = dtype == DET_DTYPE_F32 ? 4 : 8;
+  const size_t groups = !top ? 0 : nseg * kSeg / (vocab <= kSmallVocab ? vec : 32 * vec);
+  return align256(n * nseg * sizeof(float4)) + align256(n * groups * sizeof(float));
+}
+template <typename T, bool TOP>
+cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te,
+                       float temp, void* workspace, float* loss, const ScoreOut& o) {
+  const auto segments = !TOP                       ? segments_kernel<T, GROUPS_NONE>
+                        : L.vocab <= kSmallVocab ? segments_kernel<T, GROUPS_LANE>
+                                                 : segments_kernel<T, GROUPS_WARP>;
+  constexpr int kSegWarps = kSegThreads / 32;
+  const size_t smem = kSegWarps * kStageBytes<T>;
+  if (cudaError_t e = raise_smem_cap((const void*)segments, smem)) return e;
+  const long long nseg = (L.vocab + kSeg - 1) / kSeg, blocks = (L.n * nseg + kSegWarps - 1) / kSegWarps;
+  const int fit = resident_clusters((const void*)segments, 1, kSegThreads, smem);
+  Workspace ws;
+  ws.seg = static_cast<float4*>(workspace);
+  ws.gmax = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256(L.n * nseg * sizeof(float4)));
+  segments<<<(unsigned)(blocks < fit ? blocks : fit), kSegThreads, smem, s>>>(L, temp, ws, 1.0f);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  const Launch launch{s, nullptr, nullptr, true};
+  return launch_k(launch, rows_kernel<T, TOP>, dim3(L.n), dim3(TOP ? kThreads : DET_MAX_TOP), 0, L, tokens, id_bytes,
+                  te, temp, ws, loss, o, 1.0f);
 }
 cudaError_t launch_forward(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
-                           const Teacher& te, float temp, float* loss, const ScoreOut& o) {
-  cudaError_t e = cudaSuccess;
-  const cudaError_t last = by_dtype(dtype, [&](auto t) {
+                           const Teacher& te, float temp, void* workspace, float* loss, const ScoreOut& o) {
+  return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    e = o.top         ? forward_as<T, true, false>(s, L, tokens, id_bytes, te, temp, loss, o)
-        : temp == 1.0f ? forward_as<T, false, false>(s, L, tokens, id_bytes, te, temp, loss, o)
-                       : forward_as<T, false, true>(s, L, tokens, id_bytes, te, temp, loss, o);
+    return o.top ? forward_as<T, true>(s, L, tokens, id_bytes, te, temp, workspace, loss, o)
+                 : forward_as<T, false>(s, L, tokens, id_bytes, te, temp, workspace, loss, o);
   });
-  return e ? e : last;
 }
-template <typename T, bool ENTROPY, bool SCALED>
+
+template <typename T, bool ENTROPY>
 cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
                     const GradIn& in, void* out, unsigned long long out_ld) {
   constexpr int VEC = Seg<T>::VEC;
   const int nvec = (L.vocab + VEC - 1) / VEC + 1;  // one more where a row starts inside a vector
   const int step = kThreads * kGradUnroll;
-  int per = 4 * step;
+  int per = 8 * step;
   while (per > step && (long long)L.n * ((nvec + per - 1) / per) < 8 * device_sms()) per -= step;
   const int blocks = (nvec + per - 1) / per;
   for (int r = 0; r < L.n; r += 65535) {
-    grad_kernel<T, ENTROPY, SCALED><<<dim3(blocks, L.n - r < 65535 ? L.n - r : 65535), kThreads, 0, s>>>(
+    grad_kernel<T, ENTROPY><<<dim3(blocks, L.n - r < 65535 ? L.n - r : 65535), kThreads, 0, s>>>(
         L, r, per, tokens, id_bytes, te, temp, in, static_cast<T*>(out), out_ld, 1.0f);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
@@ -924,14 +1381,36 @@ cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
 }
 cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
                         const Teacher& te, float temp, const GradIn& in, void* out, unsigned long long out_ld) {
-  cudaError_t e = cudaSuccess;
-  const cudaError_t last = by_dtype(dtype, [&](auto t) {
+  return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    e = in.gh           ? grad_as<T, true, false>(s, L, tokens, id_bytes, te, temp, in, out, out_ld)
-        : temp == 1.0f ? grad_as<T, false, false>(s, L, tokens, id_bytes, te, temp, in, out, out_ld)
-                       : grad_as<T, false, true>(s, L, tokens, id_bytes, te, temp, in, out, out_ld);
+    return in.gh ? grad_as<T, true>(s, L, tokens, id_bytes, te, temp, in, out, out_ld)
+                 : grad_as<T, false>(s, L, tokens, id_bytes, te, temp, in, out, out_ld);
   });
-  return e ? e : last;
+}
+
+template <typename T, bool ENTROPY>
+cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
+                    const GradIn& in, float* loss, const ScoreOut& o, void* out, unsigned long long out_ld) {
+  const auto kern = step_kernel<T, ENTROPY>;
+  // a warp per segment; at least DET_MAX_TOP threads, one per list entry
+  const int nseg = (L.vocab + kSeg - 1) / kSeg, c = (nseg + kWarps - 1) / kWarps;
+  const int need = (nseg + c - 1) / c, warps = need < (int)DET_MAX_TOP / 32 ? (int)DET_MAX_TOP / 32 : need;
+  const size_t smem = warps * kStageBytes<T>;
+  if (cudaError_t e = raise_smem_cap((const void*)kern, smem)) return e;
+  if (c > 8)
+    if (cudaError_t e = allow_large_clusters((const void*)kern)) return e;
+  const int fit = resident_clusters((const void*)kern, c, 32 * warps, smem);
+  return launch_clusters(s, kern, L.n < fit ? L.n : fit, c, 32 * warps, smem, L, tokens, id_bytes, te, temp, in, loss,
+                         o, static_cast<T*>(out), out_ld, 1.0f);
+}
+cudaError_t launch_step(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
+                        const Teacher& te, float temp, const GradIn& in, float* loss, const ScoreOut& o, void* out,
+                        unsigned long long out_ld) {
+  return by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return in.gh ? step_as<T, true>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld)
+                 : step_as<T, false>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld);
+  });
 }
 
 // ---- argument checks ----------------------------------------------------------------
@@ -974,6 +1453,11 @@ det_status check_list(const void* ids, int id_bytes, const void* teacher, int te
   if (!(temperature >= DET_MIN_TEMPERATURE && temperature <= DET_MAX_TEMPERATURE)) return DET_ERR_INVALID_ARGUMENT;
   return DET_OK;
 }
+det_status check_workspace(const void* workspace, size_t size, int dtype, uint32_t n, uint32_t vocab, uint32_t top) {
+  if (!workspace || (uintptr_t)workspace % 16 || size < workspace_bytes(dtype, (int)n, (int)vocab, (int)top))
+    return DET_ERR_INVALID_ARGUMENT;
+  return DET_OK;
+}
 det_status check_device() {
   int cnt = 0;
   return cudaGetDeviceCount(&cnt) != cudaSuccess || cnt == 0 ? DET_ERR_NO_DEVICE : DET_OK;
@@ -988,20 +1472,23 @@ const Teacher kNoTeacher{nullptr, nullptr, 0, 4, DET_DTYPE_F32, 0};
 
 cudaError_t launch_token_scores(const Launch& L, const float* logits, int V, const uint32_t* rows,
                                 const uint32_t* tokens, int n, int top, float* logprob, float* entropy,
-                                int32_t* top_ids, float* top_logprobs) {
+                                int32_t* top_ids, float* top_logprobs, void* workspace) {
   const Logits x{logits, rows, (unsigned long long)V, n, V};
   const ScoreOut o{logprob, entropy, nullptr, top_ids, top_logprobs, top, L.err};
-  if (L.launches) ++*L.launches;
-  return launch_forward(L.stream, DET_DTYPE_F32, x, tokens, 4, kNoTeacher, 1.0f, nullptr, o);
+  if (L.launches) *L.launches += 2;
+  return launch_forward(L.stream, DET_DTYPE_F32, x, tokens, 4, kNoTeacher, 1.0f, workspace, nullptr, o);
 }
 cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, const uint32_t* rows, int n,
-                                const int32_t* ids, const float* teacher, int k, float temperature, float* loss) {
+                                const int32_t* ids, const float* teacher, int k, float temperature, float* loss,
+                                void* workspace) {
   const Logits x{logits, rows, (unsigned long long)V, n, V};
   const Teacher te{ids, teacher, (unsigned long long)k, 4, DET_DTYPE_F32, k};
   const ScoreOut o{nullptr, nullptr, nullptr, nullptr, nullptr, 0, L.err};
-  if (L.launches) ++*L.launches;
-  return launch_forward(L.stream, DET_DTYPE_F32, x, nullptr, 4, te, temperature, loss, o);
+  if (L.launches) *L.launches += 2;
+  return launch_forward(L.stream, DET_DTYPE_F32, x, nullptr, 4, te, temperature, workspace, loss, o);
 }
+
+size_t scores_workspace_bytes(int n, int V, int top) { return workspace_bytes(DET_DTYPE_F32, n, V, top); }
 
 static_assert(DET_SCORE_NONFINITE == (int)ERRF_CDF_NONFINITE && DET_SCORE_BAD_TOKEN == (int)ERRF_SYMBOL,
               "the flags are the session's error bits");
@@ -1011,20 +1498,26 @@ using namespace det;
 
 extern "C" {
 
+size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top) {
+  if (dtype < DET_DTYPE_F32 || dtype > DET_DTYPE_BF16 || vocab > kMaxVocab || n > DET_SCORE_MAX_ROWS) return 0;
+  return workspace_bytes(dtype, (int)n, (int)vocab, (int)top);
+}
+
 det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* tokens, int token_bytes, uint32_t top, float* logprob, float* entropy,
                                    float* stats, int32_t* top_ids, float* top_logprobs, uint32_t* flags,
-                                   void* stream) {
+                                   void* workspace, size_t workspace_size, void* stream) {
   if (n == 0) return DET_OK;
   if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
   if (logprob)
     if (det_status st = check_ids(tokens, token_bytes)) return st;
   if (top > DET_MAX_TOP || top > vocab || (top && !top_ids && !top_logprobs)) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_workspace(workspace, workspace_size, dtype, n, vocab, top)) return st;
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const ScoreOut o{logprob, entropy, stats, top_ids, top_logprobs, (int)top, flags};
   return launched(launch_forward(static_cast<cudaStream_t>(stream), dtype, L, tokens, token_bytes, kNoTeacher, 1.0f,
-                                 nullptr, o));
+                                 workspace, nullptr, o));
 }
 
 det_status det_token_scores_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
@@ -1056,26 +1549,26 @@ det_status det_token_scores_step_device(const void* logits, int dtype, uint32_t 
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const ScoreOut o{logprob, entropy, stats, nullptr, nullptr, 0, flags};
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaError_t e = launch_forward(s, dtype, L, tokens, token_bytes, kNoTeacher, 1.0f, nullptr, o))
-    return launched(e);
-  return launched(launch_grad(s, dtype, L, tokens, token_bytes, kNoTeacher, 1.0f,
-                              GradIn{stats, grad_logprob, grad_entropy}, grad, grad_ld));
+  return launched(launch_step(static_cast<cudaStream_t>(stream), dtype, L, logprob || grad_logprob ? tokens : nullptr,
+                              token_bytes, kNoTeacher, 1.0f, GradIn{nullptr, grad_logprob, grad_entropy}, nullptr, o,
+                              grad, grad_ld));
 }
 
 det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
                                    uint64_t list_ld, float temperature, float* loss, float* stats, uint32_t* flags,
-                                   void* stream) {
+                                   void* workspace, size_t workspace_size, void* stream) {
   if (n == 0) return DET_OK;
   if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
   if (det_status st = check_list(ids, id_bytes, teacher, teacher_dtype, k, n, list_ld, temperature)) return st;
   if (!loss) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_workspace(workspace, workspace_size, dtype, n, vocab, 0)) return st;
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
   const ScoreOut o{nullptr, nullptr, stats, nullptr, nullptr, 0, flags};
-  return launched(launch_forward(static_cast<cudaStream_t>(stream), dtype, L, nullptr, 4, te, temperature, loss, o));
+  return launched(launch_forward(static_cast<cudaStream_t>(stream), dtype, L, nullptr, 4, te, temperature,
+                                 workspace, loss, o));
 }
 
 det_status det_distill_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
@@ -1107,10 +1600,8 @@ det_status det_distill_step_device(const void* logits, int dtype, uint32_t n, ui
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
   const ScoreOut o{nullptr, nullptr, stats, nullptr, nullptr, 0, flags};
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaError_t e = launch_forward(s, dtype, L, nullptr, 4, te, temperature, loss, o)) return launched(e);
-  return launched(
-      launch_grad(s, dtype, L, nullptr, 4, te, temperature, GradIn{stats, grad_loss, nullptr}, grad, grad_ld));
+  return launched(launch_step(static_cast<cudaStream_t>(stream), dtype, L, nullptr, 4, te, temperature,
+                              GradIn{nullptr, grad_loss, nullptr}, loss, o, grad, grad_ld));
 }
 
 }  // extern "C"

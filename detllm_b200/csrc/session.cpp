@@ -969,14 +969,16 @@ det_status det_decoder_lookup(det_session* s, uint32_t row, int byte_escapes, ui
 }
 
 // ---- token scores and distillation (scoring.cu) --------------------------
-// d_score / h_score hold one group of up to 1,024 rows: 16 bytes per row
-// (token or loss, logprob, entropy) and 8 per list entry (id, value).
+// d_score / h_score hold one group of rows: 16 bytes per row (token or loss,
+// logprob, entropy) and 8 per list entry (id, value); on the device the
+// kernels' workspace follows.
 static constexpr uint32_t kScoreRows = 1024;
+static constexpr size_t kScoreBytes = (size_t)kScoreRows * (16 + 8 * DET_MAX_TOP);
 static det_status score_buffers(det_session* s) {
-  const size_t bytes = (size_t)kScoreRows * (16 + 8 * DET_MAX_TOP);
+  const int rows = std::min<int>(s->max_chunk, kScoreRows);
   if (!s->d_score)
-    if (det_status st = dalloc(s, &s->d_score, bytes)) return st;
-  return s->h_score ? DET_OK : halloc(s, &s->h_score, bytes);
+    if (det_status st = dalloc(s, &s->d_score, kScoreBytes + scores_workspace_bytes(rows, s->m->vocab, 1))) return st;
+  return s->h_score ? DET_OK : halloc(s, &s->h_score, kScoreBytes);
 }
 
 // a group's rows, checked, into h_rows (copied to the device by the caller)
@@ -998,8 +1000,9 @@ det_status det_token_scores(det_session* s, const uint32_t* rows, const uint32_t
   const uint32_t V = (uint32_t)s->m->vocab;
   cudaSetDevice(s->m->device);
   if (det_status st = score_buffers(s)) return st;
-  for (uint32_t base = 0; base < n; base += kScoreRows) {
-    const uint32_t cnt = std::min(kScoreRows, n - base);
+  const uint32_t group = std::min<uint32_t>((uint32_t)s->max_chunk, kScoreRows);
+  for (uint32_t base = 0; base < n; base += group) {
+    const uint32_t cnt = std::min(group, n - base);
     if (det_status st = score_rows(s, rows, base, cnt)) return st;
     // tokens | logprob | entropy | top logprobs | top ids
     uint32_t* ht = reinterpret_cast<uint32_t*>(s->h_score);
@@ -1016,7 +1019,7 @@ det_status det_token_scores(det_session* s, const uint32_t* rows, const uint32_t
     CK(timed(s, PT_CDF, 0, 0, [&] {
       return launch_token_scores(launch_of(s), s->logits, (int)V, s->d_rows + 1024,
                                  reinterpret_cast<const uint32_t*>(s->d_score), (int)cnt, (int)top, d, d + cnt,
-                                 reinterpret_cast<int32_t*>(d + 2 * cnt + list), d + 2 * cnt);
+                                 reinterpret_cast<int32_t*>(d + 2 * cnt + list), d + 2 * cnt, s->d_score + kScoreBytes);
     }));
     CK(cudaEventRecord(s->ev[3], s->stream));
     const size_t words = 2 * (size_t)cnt + 2 * list;
@@ -1047,8 +1050,9 @@ det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, co
   const uint32_t V = (uint32_t)s->m->vocab;
   cudaSetDevice(s->m->device);
   if (det_status st = score_buffers(s)) return st;
-  for (uint32_t base = 0; base < n; base += kScoreRows) {
-    const uint32_t cnt = std::min(kScoreRows, n - base);
+  const uint32_t group = std::min<uint32_t>((uint32_t)s->max_chunk, kScoreRows);
+  for (uint32_t base = 0; base < n; base += group) {
+    const uint32_t cnt = std::min(group, n - base);
     if (det_status st = score_rows(s, rows, base, cnt)) return st;
     // ids | values | loss
     const size_t list = (size_t)cnt * k;
@@ -1068,7 +1072,8 @@ det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, co
     float* d = reinterpret_cast<float*>(s->d_score);
     CK(timed(s, PT_CDF, 0, 0, [&] {
       return launch_distill_loss(launch_of(s), s->logits, (int)V, s->d_rows + 1024, (int)cnt,
-                                 reinterpret_cast<const int32_t*>(d), d + list, (int)k, temperature, d + 2 * list);
+                                 reinterpret_cast<const int32_t*>(d), d + list, (int)k, temperature, d + 2 * list,
+                                 s->d_score + kScoreBytes);
     }));
     CK(cudaEventRecord(s->ev[3], s->stream));
     CK(cudaMemcpyAsync(s->h_score, d + 2 * list, cnt * 4, cudaMemcpyDeviceToHost, s->stream));

@@ -107,6 +107,11 @@ def _new(logits, *shape):
     return torch.empty(shape, dtype=torch.float32, device=logits.device)
 
 
+def _workspace(logits, n, vocab, top):
+    size = lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, top)
+    return torch.empty(size, dtype=torch.uint8, device=logits.device), size
+
+
 def token_scores(logits, tokens, top: int = 0) -> TokenScores:
     """Log probability of ``tokens[i]`` under row i, the row's entropy, and its
     ``top`` (at most 128) most likely tokens, most likely first and equal ones
@@ -120,9 +125,10 @@ def token_scores(logits, tokens, top: int = 0) -> TokenScores:
             raise ValueError("top must not be negative")
         ids = torch.empty((n, top), dtype=torch.int32, device=logits.device)
         lps = _new(logits, n, top)
+    work, size = _workspace(logits, n, vocab, top)
     _call("det_token_scores_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
           _IDS[tokens.dtype], top, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
-          ids.data_ptr() if top else None, lps.data_ptr() if top else None, None)
+          ids.data_ptr() if top else None, lps.data_ptr() if top else None, None, work.data_ptr(), size)
     return TokenScores(logprob, entropy, stats, ids, lps)
 
 
@@ -165,8 +171,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) 
     n, vocab, ld = _logits(logits)
     lists = _lists(teacher_ids, teacher_logits, logits, n)
     loss, stats = _new(logits, n), _new(logits, n, 4)
+    work, size = _workspace(logits, n, vocab, 0)
     _call("det_distill_loss_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
-          temperature, loss.data_ptr(), stats.data_ptr(), None)
+          temperature, loss.data_ptr(), stats.data_ptr(), None, work.data_ptr(), size)
     return DistillLoss(loss, stats)
 
 

@@ -325,10 +325,11 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  *   an id listed twice         two terms of the loss; its gradient has both
  * A probability below exp(-88) of the row's largest counts as 0.
  *
- * Results are deterministic, and a row's are the same bits in whatever batch,
- * stride or call it is (the sums' order depends on the vocabulary and the
- * element type alone).  They are not specified bit for bit across library
- * versions.
+ * Results are deterministic, and a row's are the same bits in whatever batch
+ * or stride it is (the order of its sums depends on the vocabulary and the
+ * element type alone); the gradients of a _step call and of a _grad call may
+ * differ in their last bits, everything else agrees between calls.  They are
+ * not specified bit for bit across library versions.
  *
  * The *_device calls work on the caller's device memory, on `stream` of the
  * calling thread's current device.  They allocate nothing, keep nothing and
@@ -360,12 +361,17 @@ det_status det_token_scores(det_session* s, const uint32_t* rows, const uint32_t
                             float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs);
 det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, const uint32_t* teacher_ids,
                             const float* teacher_logits, uint32_t k, float temperature, float* loss);
+/* bytes of workspace that det_token_scores_device (and, with top = 0,
+ * det_distill_loss_device) needs; 16-byte aligned.  Calls that may overlap
+ * need one each; what it holds between calls does not matter. */
+size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top);
 /* log probability of tokens[i], entropy, and the `top` (<= DET_MAX_TOP, <=
  * vocab) most likely tokens of row i with their log probabilities, most
  * likely first, equal ones in the order of their ids: n x top each */
 det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* tokens, int token_bytes, uint32_t top, float* logprob, float* entropy,
-                                   float* stats, int32_t* top_ids, float* top_logprobs, uint32_t* flags, void* stream);
+                                   float* stats, int32_t* top_ids, float* top_logprobs, uint32_t* flags,
+                                   void* workspace, size_t workspace_size, void* stream);
 /* grad = d (sum_i grad_logprob[i] logprob[i] + grad_entropy[i] entropy[i]) /
  * d logits; either of the two may be NULL */
 det_status det_token_scores_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
@@ -382,7 +388,7 @@ det_status det_token_scores_step_device(const void* logits, int dtype, uint32_t 
 det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
                                    uint64_t list_ld, float temperature, float* loss, float* stats, uint32_t* flags,
-                                   void* stream);
+                                   void* workspace, size_t workspace_size, void* stream);
 /* grad = d (sum_i grad_loss[i] loss[i]) / d logits (the teacher has none) */
 det_status det_distill_grad_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,

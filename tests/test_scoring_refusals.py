@@ -20,8 +20,8 @@ def lib():
     return D.lib()
 
 
-def scores(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, tok=P, tb=8, top=0, lp=P, en=P, st=P, ids=None, lps=None):
-    return lib.det_token_scores_device(x, dtype, n, vocab, ld, tok, tb, top, lp, en, st, ids, lps, None, None)
+def scores(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, tok=P, tb=8, top=0, lp=P, en=P, st=P, ids=None, lps=None, ws=P, size=1 << 40):
+    return lib.det_token_scores_device(x, dtype, n, vocab, ld, tok, tb, top, lp, en, st, ids, lps, None, ws, size, None)
 
 
 def scores_grad(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, tok=P, tb=8, st=P, gl=P, ge=None, out=P, old=1000):
@@ -33,8 +33,10 @@ def scores_step(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, tok=P, tb=8, gl=P
     return lib.det_token_scores_step_device(x, dtype, n, vocab, ld, tok, tb, gl, ge, lp, en, st, out, old, None, None)
 
 
-def loss(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, ids=P, ib=4, u=P, ud=F32, k=8, lld=8, t=1.0, out=P, st=P):
-    return lib.det_distill_loss_device(x, dtype, n, vocab, ld, ids, ib, u, ud, k, lld, t, out, st, None, None)
+def loss(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, ids=P, ib=4, u=P, ud=F32, k=8, lld=8, t=1.0, out=P, st=P,
+         ws=P, size=1 << 40):
+    return lib.det_distill_loss_device(x, dtype, n, vocab, ld, ids, ib, u, ud, k, lld, t, out, st, None, ws, size,
+                                       None)
 
 
 def loss_grad(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, ids=P, ib=4, u=P, ud=F32, k=8, lld=8, t=1.0, st=P, g=P,
@@ -93,6 +95,19 @@ def test_top(lib):
     assert scores(lib, top=128, ids=P, lps=P) == NO_DEVICE
     assert scores(lib, top=129, ids=P, lps=P) == INVALID
     assert scores(lib, top=6, vocab=5, ids=P, lps=P) == INVALID
+
+
+@pytest.mark.parametrize("call", [scores, loss])
+def test_workspace(lib, call):
+    need = lib.det_scores_workspace(F32, 4, 1000, 0)
+    assert need > 0
+    assert call(lib, size=need) == NO_DEVICE
+    assert call(lib, size=need - 1) == INVALID
+    assert call(lib, ws=None) == INVALID
+    assert call(lib, ws=P + 8) == INVALID
+    assert lib.det_scores_workspace(F32, 4, 1000, 5) > need  # a top list keeps more
+    assert lib.det_scores_workspace(F32, 4, (1 << 18) + 1, 0) == 0
+    assert lib.det_scores_workspace(3, 4, 1000, 0) == 0
 
 
 @pytest.mark.parametrize("call", LISTS)
