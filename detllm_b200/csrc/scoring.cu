@@ -80,31 +80,35 @@ DI float max_nan(float a, float b) {  // NaN if either is
   return r;
 }
 
-// 2^y for y <= 0, two at a time, by Tang's table-driven method: y = k + i/32 +
-// f with |f| <= 1/64 (a rounding to a multiple of 1/32 by adding 1.5 * 2^18),
-// 2^f by a degree-2 minimax polynomial (relative error 0.9 * 2^-24), 2^(i/32)
-// from a table of 32 that a warp holds one entry per lane and reads with a
-// shuffle (no two lanes conflict), 2^k added to the entry's exponent field.
-// 13 rounded f32 operations per entry of a row with its two sums, against 19
-// for a degree-5 polynomial on |f| <= 1/2: the f32 pipe bounds the passes over
-// 16-bit logits, while the shuffle and the integer operations run beside it.
-// Within 3.8 * 2^-24 of 2^y for y >= -126.  At kYLow the result is +0 (the
-// exponent field goes negative there and the integer maximum clears it).  NaN
-// gives an unspecified number: callers keep y, which stays NaN, beside it.
+// 2^y for y <= 0, two at a time, after Tang's table-driven method: y = k + i/32
+// + f with |f| <= 1/64 (a rounding to a multiple of 1/32 by adding 1.5 * 2^18);
+// 2^f as a square, A ((f + B)^2 + D), where B = 46/32 is near 1 / ln 2 and a
+// multiple of 1/32, so f + B is one addition (maximal relative error 3.6 *
+// 2^-24 with A and D for it that make 2^0 exactly 1; 0.9 with the best B,
+// which takes two operations more); A 2^(i/32) from a table of 32 that a warp
+// holds one entry per lane and reads with a shuffle (no two lanes conflict);
+// 2^k added to the entry's exponent field.  11 rounded f32 operations for an
+// entry of a row with its two sums, against 19 for a degree-5 polynomial on
+// |f| <= 1/2: issue slots (two for a packed operation) bound the passes over
+// 16-bit logits.
+// Within 7.1 * 2^-24 of 2^y where that is 2^-122 or more, and 0 below 2^-123.
+// NaN gives an unspecified number: callers keep y, which stays NaN, beside it.
 constexpr float kYLow = -127.5f;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147182f;
-// bits of 2^(i/32), less i << 18: adding (32 k + i) << 18 leaves 2^(k + i/32)
+constexpr float kExpB = 1.4375f, kExpD = 2.0812597f;
+// bits of 0.24109945 * 2^(i/32), less i << 18: adding (32 k + i) << 18 leaves
+// those of 0.24109945 * 2^(k + i/32)
 static __device__ const uint32_t kExpTable[32] = {
-    0x3f800000u, 0x3f7ecd87u, 0x3f7daac3u, 0x3f7c980fu, 0x3f7b95c2u, 0x3f7aa43au, 0x3f79c3d3u, 0x3f78f4f0u,
-    0x3f7837f0u, 0x3f778d3au, 0x3f76f532u, 0x3f767043u, 0x3f75fed7u, 0x3f75a15bu, 0x3f75583fu, 0x3f7523f6u,
-    0x3f7504f3u, 0x3f74fbafu, 0x3f7508a4u, 0x3f752c4du, 0x3f75672au, 0x3f75b9beu, 0x3f76248cu, 0x3f76a81eu,
-    0x3f7744fdu, 0x3f77fbb8u, 0x3f78ccdfu, 0x3f79b907u, 0x3f7ac0c7u, 0x3f7be4bau, 0x3f7d257du, 0x3f7e83b3u,
+    0x3e76e2c6u, 0x3e784abcu, 0x3e78e880u, 0x3e77bb1eu, 0x3e769d8fu, 0x3e75902bu, 0x3e74934du, 0x3e73a752u,
+    0x3e72cc98u, 0x3e720381u, 0x3e714c6eu, 0x3e70a7c5u, 0x3e7015eeu, 0x3e6f9751u, 0x3e6f2c5bu, 0x3e6ed579u,
+    0x3e6e931cu, 0x3e6e65b8u, 0x3e6e4dc1u, 0x3e6e4bb0u, 0x3e6e6000u, 0x3e6e8b2eu, 0x3e6ecdbau, 0x3e6f2828u,
+    0x3e6f9afcu, 0x3e7026c1u, 0x3e70cc01u, 0x3e718b4cu, 0x3e726533u, 0x3e735a4cu, 0x3e746b2fu, 0x3e759878u,
 };
 struct Exp2 {
   f2 e, y;  // 2^y, and y as clamped
 };
 struct ExpParts {
-  f2 z, p, y;  // magic + (32 k + i) / 32, 2^f, the clamped argument
+  f2 z, p, y;  // 1.5 * 2^18 + (32 k + i) / 32, 2^f / A, the clamped argument
 };
 template <bool CLAMP>
 DI ExpParts exp_parts(f2 y, f2 one) {
@@ -114,20 +118,21 @@ DI ExpParts exp_parts(f2 y, f2 one) {
     c.y = max_nan(c.y, kYLow);
     y = pk(c.x, c.y);
   }
-  const f2 magic = pk(393216.0f, 393216.0f), neg = pk(-1.0f, -1.0f);
+  const f2 magic = pk(393216.0f, 393216.0f), shifted_magic = pk(393216.0f + kExpB, 393216.0f + kExpB);
+  const f2 neg = pk(-1.0f, -1.0f);
   const f2 z = addp(y, one, magic);  // y may come straight from a multiply
-  const f2 f = addp(y, one, fma2(z, neg, magic));  // magic - z: an exact multiply by -1
-  const f2 q = addp(mul2(pk(0.24022649f, 0.24022649f), f), one, pk(0.6931573f, 0.6931573f));
-  return {z, addp(mul2(q, f), one, pk(1.0f, 1.0f)), y};
+  const f2 g = addp(y, one, fma2(z, neg, shifted_magic));  // an exact multiply by -1; f + B
+  return {z, addp(mul2(g, g), one, pk(kExpD, kExpD)), y};
 }
+// the table's entry times 2^k; CLAMP: 0 where that is not a normal number
 template <bool CLAMP>
 DI float exp_scale(uint32_t entry, float z) {
   const int b = (int)(entry + (__float_as_uint(z) << 18));
-  return __int_as_float(CLAMP ? max(b, 0) : b);
+  return __int_as_float(CLAMP && b < 0x00800000 ? 0 : b);
 }
 // every lane of the warp takes part; `table`: the lane's entry.  Without CLAMP
 // every y that is a number has to be >= kYSafe; the bits are the same.
-constexpr float kYSafe = -126.0f;
+constexpr float kYSafe = -122.0f;
 template <bool CLAMP>
 DI Exp2 exp2_warp(f2 y, uint32_t table, f2 one) {
   const ExpParts t = exp_parts<CLAMP>(y, one);
@@ -193,6 +198,29 @@ DI void unpack_vec(uint4 w, float* v) {
         v[2 * i] = f.x;
         v[2 * i + 1] = f.y;
       }
+    }
+  }
+}
+// x + c for the pairs of a vector: a 16-bit x is widened by the addition itself
+template <typename T>
+DI void add_vec(uint4 w, float c, f2 (&d)[8 / sizeof(T)]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (std::is_same_v<T, float>) {
+    d[0] = add2(pk(__uint_as_float(u[0]), __uint_as_float(u[1])), pk(c, c));
+    d[1] = add2(pk(__uint_as_float(u[2]), __uint_as_float(u[3])), pk(c, c));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const unsigned short lo = (unsigned short)u[i], hi = (unsigned short)(u[i] >> 16);
+      float a, b;
+      if constexpr (std::is_same_v<T, __half>) {
+        asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(a) : "h"(lo), "f"(c));
+        asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(b) : "h"(hi), "f"(c));
+      } else {
+        asm("add.rn.f32.bf16 %0, %1, %2;" : "=f"(a) : "h"(lo), "f"(c));
+        asm("add.rn.f32.bf16 %0, %1, %2;" : "=f"(b) : "h"(hi), "f"(c));
+      }
+      d[i] = pk(a, b);
     }
   }
 }
@@ -315,23 +343,52 @@ DI void stage_take(const void* buf, int mis, uint4 (&v)[Seg<T>::NV]) {
   }
   __syncwarp();
 }
-// largest and smallest entry of a vector; NaN loses against a number
+DI float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+DI float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The largest and smallest of vectors' entries, taken vector by vector; NaN
+// loses against a number.
 template <typename T>
-DI void vec_range(uint4 w, float& hi, float& lo) {
-  if constexpr (std::is_same_v<T, float>) {
-    const float a = __uint_as_float(w.x), b = __uint_as_float(w.y), c = __uint_as_float(w.z), d = __uint_as_float(w.w);
-    hi = fmaxf(fmaxf(a, b), fmaxf(c, d));
-    lo = fminf(fminf(a, b), fminf(c, d));
-  } else {
-    using P = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+struct Range {
+  float hi = -INFINITY, lo = INFINITY;
+  DI void take(uint4 w) {
+    hi = max3(max3(hi, __uint_as_float(w.x), __uint_as_float(w.y)), __uint_as_float(w.z), __uint_as_float(w.w));
+    lo = min3(min3(lo, __uint_as_float(w.x), __uint_as_float(w.y)), __uint_as_float(w.z), __uint_as_float(w.w));
+  }
+  DI float high() const { return hi; }
+  DI float low() const { return lo; }
+};
+template <typename P>  // pairs of 16-bit entries
+struct PairRange {
+  P hi, lo;
+  DI PairRange() {
+    const uint32_t inf = std::is_same_v<P, __half2> ? 0x7c007c00u : 0x7f807f80u, ninf = inf | 0x80008000u;
+    memcpy(&hi, &ninf, 4);
+    memcpy(&lo, &inf, 4);
+  }
+  DI void take(uint4 w) {
     P p[4];
     memcpy(p, &w, 16);
-    const P h = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
-    const P l = __hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3]));
-    hi = to_f32(__hmax(h.x, h.y));
-    lo = to_f32(__hmin(l.x, l.y));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      hi = __hmax2(hi, p[i]);
+      lo = __hmin2(lo, p[i]);
+    }
   }
-}
+  DI float high() const { return fmaxf(to_f32(hi.x), to_f32(hi.y)); }
+  DI float low() const { return fminf(to_f32(lo.x), to_f32(lo.y)); }
+};
+template <>
+struct Range<__half> : PairRange<__half2> {};
+template <>
+struct Range<__nv_bfloat16> : PairRange<__nv_bfloat162> {};
 
 struct Sums {
   float m, s, w;  // maximum, sum of 2^y, sum of 2^y y, with y = (x - m) log2(e) / T
@@ -366,7 +423,7 @@ DI float sum_segment(const uint4 (&v)[Seg<T>::NV], int entries, float m, float c
                      float* e) {
   using G = Seg<T>;
   const float base = m == -INFINITY ? 0.0f : -m;
-  const f2 nm = pk(base, base), one = pk(one_, one_), cc = pk(c, c);
+  const f2 one = pk(one_, one_), cc = pk(c, c);
   f2 s[2] = {0, 0}, w[2] = {0, 0};
 #pragma unroll
   for (int q = 0; q < 4; q++) {
@@ -379,11 +436,11 @@ DI float sum_segment(const uint4 (&v)[Seg<T>::NV], int entries, float m, float c
     }
 #pragma unroll
     for (int i = q * (G::NV / 4); i < (q + 1) * (G::NV / 4); i++) {
-      float x[G::VEC];
-      unpack_vec<T>(v[i], x);
+      f2 d[G::VEC / 2];
+      add_vec<T>(v[i], base, d);
 #pragma unroll
       for (int j = 0; j < G::VEC / 2; j++) {
-        const Exp2 t = exp2_warp<CLAMP>(mul2(add2(pk(x[2 * j], x[2 * j + 1]), nm), cc), table, one);
+        const Exp2 t = exp2_warp<CLAMP>(mul2(d[j], cc), table, one);
         s[j & 1] = add2(s[j & 1], t.e);
         w[j & 1] = addp(mul2(t.e, t.y), one, w[j & 1]);
         if constexpr (KEEP) {
@@ -399,7 +456,7 @@ DI float sum_segment(const uint4 (&v)[Seg<T>::NV], int entries, float m, float c
 }
 // `low`: the smallest entry.  Where no entry is so far below the maximum that
 // its power has to be cleared, the clamp and the clearing are left out (4
-// integer-pipe operations of 23 per pair of entries).
+// of some 20 operations per pair of entries).
 template <typename T, bool KEEP>
 DI float segment_sums(const uint4 (&v)[Seg<T>::NV], int entries, float m, float low, float c, uint32_t table,
                       float one, float* e) {
@@ -835,15 +892,17 @@ __global__ void __launch_bounds__(kSegThreads, kSegBlocks)
     int nrow = row + drow, ng = g + dg;
     if (ng >= nseg) ng -= nseg, nrow++;
     if (nrow < L.n) stage_issue<T>(stage, at_row(nrow), ng, V);
-    float m = -INFINITY, low = INFINITY, gm = -INFINITY;
+    Range<T> all_range;
+    float gm = -INFINITY;
     const size_t part = (size_t)row * nseg + g;
     float* gmax = ws.gmax + part * (kSeg / G::VEC) + l;
 #pragma unroll
     for (int i = 0; i < G::NV; i++) {
-      float lm, ll;
-      vec_range<T>(v[i], lm, ll);
-      m = fmaxf(m, lm);
-      low = fminf(low, ll);
+      all_range.take(v[i]);
+      if constexpr (GROUPS == GROUPS_NONE) continue;
+      Range<T> group;
+      group.take(v[i]);
+      const float lm = group.high();
       if constexpr (GROUPS == GROUPS_LANE) gmax[i * 32] = lm;
       if constexpr (GROUPS == GROUPS_WARP) {
         const float r = redux_max(lm);
@@ -853,8 +912,7 @@ __global__ void __launch_bounds__(kSegThreads, kSegBlocks)
     if constexpr (GROUPS == GROUPS_WARP) {
       if (l < G::NV) ws.gmax[part * G::NV + l] = gm;
     }
-    m = redux_max(m);
-    low = redux_min(low);
+    const float m = redux_max(all_range.high()), low = redux_min(all_range.low());
     const float s = segment_sums<T, false>(v, V - g * kSeg, m, low, c, table, one, nullptr);
     const float w = __shfl_sync(kFull, s, 16);
     if (l == 0) ws.seg[part] = make_float4(m, s, w, 0.0f);
@@ -1019,7 +1077,7 @@ __global__ void __launch_bounds__(kThreads, 3)
   float mine = 0.0f;
   if (patch) mine = fadd(grad1<ENTROPY>(to_f32(x[id]), r, one_), add);
   __syncthreads();
-  const f2 one = pk(one_, one_), base = pk(r.base, r.base), cc = pk(c, c);
+  const f2 one = pk(one_, one_), cc = pk(c, c);
   for (int b = q0; b < q1; b += kThreads * U) {  // the same turns for all lanes: exp2_warp shuffles
     const int q = b + threadIdx.x;
     uint4 next[U];
@@ -1028,29 +1086,31 @@ __global__ void __launch_bounds__(kThreads, 3)
     fetch(q + kThreads * U, next);
     // no entry of the warp is so far below the maximum that it has to be
     // cleared (vectors that are not whole are left out: not safe)
-    float low = INFINITY, high;
+    Range<T> range;
+    bool part = false;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      float lo;
-      vec_range<T>(cur[u], high, lo);
-      const bool in_row = q + u * kThreads < q1;
-      low = fminf(low, !in_row ? INFINITY : whole((q + u * kThreads) * VEC - my) ? lo : -INFINITY);
+      if (q + u * kThreads >= q1) continue;
+      range.take(cur[u]);
+      part |= !whole((q + u * kThreads) * VEC - my);
     }
-    const bool safe = fmul(fadd(redux_min(low), r.base), c) >= kYSafe;
+    const bool safe = fmul(fadd(redux_min(part ? -INFINITY : range.low()), r.base), c) >= kYSafe;
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int at = (q + u * kThreads) * VEC - my;
       const bool in_row = q + u * kThreads < q1;
       float v[VEC];
-      unpack_vec<T>(cur[u], v);
       if (in_row && !whole(at)) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) v[j] = at + j >= 0 && at + j < V ? to_f32(x[at + j]) : 0.0f;
+        cur[u] = pack_vec<T>(v);
       }
+      f2 d[VEC / 2];
+      add_vec<T>(cur[u], r.base, d);
       if (safe) {
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
-          const Exp2 e = exp2_warp<false>(mul2(add2(pk(v[j], v[j + 1]), base), cc), table, one);
+          const Exp2 e = exp2_warp<false>(mul2(d[j / 2], cc), table, one);
           const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
           v[j] = gr.x;
           v[j + 1] = gr.y;
@@ -1058,7 +1118,7 @@ __global__ void __launch_bounds__(kThreads, 3)
       } else {
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
-          const Exp2 e = exp2_warp<true>(mul2(add2(pk(v[j], v[j + 1]), base), cc), table, one);
+          const Exp2 e = exp2_warp<true>(mul2(d[j / 2], cc), table, one);
           const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
           v[j] = gr.x;
           v[j + 1] = gr.y;
@@ -1159,16 +1219,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (active) {
       stage_take<T>(stage, misaligned(x), raw);
       if (row + clusters < L.n) stage_issue<T>(stage, at_row(row + clusters), g, V);
-      float low = INFINITY;
+      Range<T> range;
 #pragma unroll
-      for (int i = 0; i < Seg<T>::NV; i++) {
-        float h, l;
-        vec_range<T>(raw[i], h, l);
-        m_seg = fmaxf(m_seg, h);
-        low = fminf(low, l);
-      }
-      m_seg = redux_max(m_seg);
-      s_seg = segment_sums<T, !ENTROPY>(raw, V - g * kSeg, m_seg, redux_min(low), c, table, one_, v);
+      for (int i = 0; i < Seg<T>::NV; i++) range.take(raw[i]);
+      m_seg = redux_max(range.high());
+      s_seg = segment_sums<T, !ENTROPY>(raw, V - g * kSeg, m_seg, redux_min(range.low()), c, table, one_, v);
       w_seg = __shfl_sync(kFull, s_seg, 16);
       s_seg = __shfl_sync(kFull, s_seg, 0);
     }
@@ -1216,18 +1271,19 @@ __global__ void __launch_bounds__(kThreads, 2)
       rg = score_grad(in, row, V, t, r.m, r.s, r.s1, c, &add);
     }
     if (active) {
-      const f2 one = pk(one_, one_), base = pk(rg.base, rg.base), cc = pk(c, c);
+      const f2 one = pk(one_, one_), cc = pk(c, c);
       const float f = fmul(exp2_one(segment_y(m_seg, r.m, c), one_), rg.as);
       // vector i of the segment's gradient
       auto vec = [&](int i) {
         constexpr int VEC = Seg<T>::VEC;
         float x[VEC];
-        if constexpr (ENTROPY) unpack_vec<T>(raw[i], x);
+        f2 dx[VEC / 2];
+        if constexpr (ENTROPY) add_vec<T>(raw[i], rg.base, dx);
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
           f2 d;
           if constexpr (ENTROPY) {
-            const Exp2 ex = exp2_warp<true>(mul2(add2(pk(x[j], x[j + 1]), base), cc), table, one);
+            const Exp2 ex = exp2_warp<true>(mul2(dx[j / 2], cc), table, one);
             d = grad2<true>(ex.e, ex.y, rg, one);
           } else {
             d = mul2(pk(v[i * VEC + j], v[i * VEC + j + 1]), pk(f, f));

@@ -323,7 +323,7 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  *   list entry: id < 0, u -inf not a valid entry; u NaN or +inf: as a bad id
  *   no valid entry in a list   loss 0 and gradient 0, whatever the logits
  *   an id listed twice         two terms of the loss; its gradient has both
- * A probability below exp(-88) of the row's largest counts as 0.
+ * A probability below 2^-123 of the row's largest counts as 0.
  *
  * Results are deterministic, and a row's are the same bits in whatever batch
  * or stride it is (the order of its sums depends on the vocabulary and the
