@@ -1014,50 +1014,58 @@ DI float grad1(float x, const RowGrad& r, float one) {
 }
 
 // Blocks (blockIdx.x) of a row (blockIdx.y + row0) take `per` of its 16-byte
-// vectors each; a vector is one of the gradient's, so that stores are whole
-// wherever the row starts.  The next vectors are loaded before these are
-// worked on, the first ones before the row's coefficients are known.  `out`
-// may be the logits themselves.
-constexpr int kGradUnroll = 4;
+// vectors each, their warps runs of 32 U vectors in turn; a vector is one of
+// the gradient's, so that stores are whole wherever the row starts.  The next
+// run is loaded before this one is worked on, the first before the row's
+// coefficients are known.  `out` may be the logits themselves.
+constexpr int kGradUnroll = 4, kGradRun = 32 * kGradUnroll;
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, 3)
     grad_kernel(Logits L, int row0, int per, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in,
                 T* out, unsigned long long out_ld, float one_) {
   constexpr int VEC = Seg<T>::VEC, U = kGradUnroll;
   __shared__ ListShared sh;
-  const int row = row0 + blockIdx.y, V = L.vocab;
+  const int row = row0 + blockIdx.y, V = L.vocab, l = threadIdx.x & 31;
   const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
   T* y = out + (size_t)row * out_ld;
   const int my = misaligned(y), mis = (misaligned(x) - my) & (VEC - 1);
   const int nvec = (V + my + VEC - 1) / VEC;
   const int q0 = blockIdx.x * per, q1 = min(nvec, q0 + per);
-  auto whole = [&](int at) { return at >= 0 && at + VEC <= V; };
+  // the run at vector q: are all its entries, and the granules they come from, in the row and the block
+  auto inside = [&](int q) {
+    const int at = q * VEC - my;
+    return q + kGradRun <= q1 && at >= mis && at + kGradRun * VEC + (mis ? VEC - mis : 0) <= V;
+  };
   auto fetch = [&](int q, uint4(&w)[U]) {
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int at = (q + u * kThreads) * VEC - my;
-      if (q + u * kThreads >= q1 || !whole(at)) continue;
-      const T* p = x + at;
+    const T* p = x + (q + l) * VEC - my;
+    if (inside(q)) {
       if (mis == 0) {
-        w[u] = *reinterpret_cast<const uint4*>(p);
-      } else if (at >= mis && at - mis + 2 * VEC <= V) {
-        const uint4* g = reinterpret_cast<const uint4*>(p - mis);
-        w[u] = shifted(g[0], g[1], mis * (int)sizeof(T));
-      } else {
-        float v[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; j++) v[j] = to_f32(p[j]);
-        w[u] = pack_vec<T>(v);
+        for (int u = 0; u < U; u++) w[u] = *reinterpret_cast<const uint4*>(p + 32 * u * VEC);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const uint4* g = reinterpret_cast<const uint4*>(p - mis + 32 * u * VEC);
+          w[u] = shifted(g[0], g[1], mis * (int)sizeof(T));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int v = q + 32 * u + l, at = v * VEC - my;
+        float f[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) f[j] = v < q1 && at + j >= 0 && at + j < V ? to_f32(x[at + j]) : 0.0f;
+        w[u] = pack_vec<T>(f);
       }
     }
   };
+  const int w = threadIdx.x >> 5;
   uint4 cur[U];
-#pragma unroll
-  for (int u = 0; u < U; u++) cur[u] = make_uint4(0, 0, 0, 0);
-  fetch(q0 + threadIdx.x, cur);
+  if (q0 + w * kGradRun < q1) fetch(q0 + w * kGradRun, cur);
   const float* st = in.stats + (size_t)row * 4;
   const float m = st[0], s = st[1], c = fdiv(kLog2e, temp);
-  const uint32_t table = kExpTable[threadIdx.x & 31];
+  const uint32_t table = kExpTable[l];
   RowGrad r;
   int id;
   float add;
@@ -1078,62 +1086,56 @@ __global__ void __launch_bounds__(kThreads, 3)
   if (patch) mine = fadd(grad1<ENTROPY>(to_f32(x[id]), r, one_), add);
   __syncthreads();
   const f2 one = pk(one_, one_), cc = pk(c, c);
-  for (int b = q0; b < q1; b += kThreads * U) {  // the same turns for all lanes: exp2_warp shuffles
-    const int q = b + threadIdx.x;
-    uint4 next[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) next[u] = make_uint4(0, 0, 0, 0);
-    fetch(q + kThreads * U, next);
-    // no entry of the warp is so far below the maximum that it has to be
-    // cleared (vectors that are not whole are left out: not safe)
-    Range<T> range;
-    bool part = false;
+  auto run = [&](uint4(&v)[U], auto clamp) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if (q + u * kThreads >= q1) continue;
-      range.take(cur[u]);
-      part |= !whole((q + u * kThreads) * VEC - my);
-    }
-    const bool safe = fmul(fadd(redux_min(part ? -INFINITY : range.low()), r.base), c) >= kYSafe;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int at = (q + u * kThreads) * VEC - my;
-      const bool in_row = q + u * kThreads < q1;
-      float v[VEC];
-      if (in_row && !whole(at)) {
-#pragma unroll
-        for (int j = 0; j < VEC; j++) v[j] = at + j >= 0 && at + j < V ? to_f32(x[at + j]) : 0.0f;
-        cur[u] = pack_vec<T>(v);
-      }
       f2 d[VEC / 2];
-      add_vec<T>(cur[u], r.base, d);
-      if (safe) {
+      add_vec<T>(v[u], r.base, d);
+      float f[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          const Exp2 e = exp2_warp<false>(mul2(d[j / 2], cc), table, one);
-          const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
-          v[j] = gr.x;
-          v[j + 1] = gr.y;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          const Exp2 e = exp2_warp<true>(mul2(d[j / 2], cc), table, one);
-          const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
-          v[j] = gr.x;
-          v[j + 1] = gr.y;
-        }
+      for (int j = 0; j < VEC / 2; j++) {
+        const Exp2 e = exp2_warp<decltype(clamp)::value>(mul2(d[j], cc), table, one);
+        const float2 gr = un(grad2<ENTROPY>(e.e, e.y, r, one));
+        f[2 * j] = gr.x;
+        f[2 * j + 1] = gr.y;
       }
-      if (r.zero) {
+      v[u] = pack_vec<T>(f);
+    }
+  };
+  for (int q = q0 + w * kGradRun; q < q1; q += kThreads * U) {
+    uint4 next[U];
+    if (q + kThreads * U < q1) fetch(q + kThreads * U, next);
+    const bool in = inside(q);
+    // is no entry so far below the maximum that its power has to be cleared
+    Range<T> range;
 #pragma unroll
-        for (int j = 0; j < VEC; j++) v[j] = 0.0f;
-      }
-      if (in_row && whole(at)) {
-        *reinterpret_cast<uint4*>(y + at) = pack_vec<T>(v);
-      } else if (in_row) {
+    for (int u = 0; u < U; u++) range.take(cur[u]);
+    if (in && fmul(fadd(redux_min(range.low()), r.base), c) >= kYSafe && !r.zero) {
+      run(cur, std::false_type{});
+    } else if (!r.zero) {
+      run(cur, std::true_type{});
+    } else {
 #pragma unroll
-        for (int j = 0; j < VEC; j++)
-          if (at + j >= 0 && at + j < V) y[at + j] = from_f32<T>(v[j]);
+      for (int u = 0; u < U; u++) cur[u] = make_uint4(0, 0, 0, 0);
+    }
+    T* p = y + (q + l) * VEC - my;
+    if (in) {
+#pragma unroll
+      for (int u = 0; u < U; u++) *reinterpret_cast<uint4*>(p + 32 * u * VEC) = cur[u];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int v = q + 32 * u + l, at = v * VEC - my;
+        if (v >= q1) continue;
+        if (at >= 0 && at + VEC <= V) {
+          *reinterpret_cast<uint4*>(y + at) = cur[u];
+        } else {
+          float f[VEC];
+          unpack_vec<T>(cur[u], f);
+#pragma unroll
+          for (int j = 0; j < VEC; j++)
+            if (at + j >= 0 && at + j < V) y[at + j] = from_f32<T>(f[j]);
+        }
       }
     }
 #pragma unroll
@@ -1424,9 +1426,11 @@ cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
                     const GradIn& in, void* out, unsigned long long out_ld) {
   constexpr int VEC = Seg<T>::VEC;
   const int nvec = (L.vocab + VEC - 1) / VEC + 1;  // one more where a row starts inside a vector
+  // up to 8 runs per warp, fewer where that would leave SMs without a block
   const int step = kThreads * kGradUnroll;
   int per = 8 * step;
   while (per > step && (long long)L.n * ((nvec + per - 1) / per) < 8 * device_sms()) per -= step;
+  while (per > kGradRun && (long long)L.n * ((nvec + per - 1) / per) < device_sms()) per /= 2;
   const int blocks = (nvec + per - 1) / per;
   for (int r = 0; r < L.n; r += 65535) {
     grad_kernel<T, ENTROPY><<<dim3(blocks, L.n - r < 65535 ? L.n - r : 65535), kThreads, 0, s>>>(
