@@ -242,29 +242,6 @@ DI uint4 shifted(uint4 a, uint4 b, int bytes) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// VEC entries from entry `at` of a row; what is past its end is -inf.  Only
-// 16-byte granules that lie in the row as a whole are loaded as such: a row
-// that starts `mis` entries into a granule takes two of them per vector.
-// RO: nothing writes the row while the kernel runs.
-template <bool RO>
-DI uint4 load16(const uint4* p) {
-  if constexpr (RO) return __ldg(p);
-  else return *p;
-}
-template <typename T, bool RO = true>
-DI void load_vec(const T* row, int at, int V, int mis, float* v) {
-  constexpr int VEC = Seg<T>::VEC;
-  const T* p = row + at;
-  if (mis == 0 && at >= 0 && at + VEC <= V) {
-    unpack_vec<T>(load16<RO>(reinterpret_cast<const uint4*>(p)), v);
-  } else if (mis != 0 && at >= mis && at - mis + 2 * VEC <= V) {
-    const uint4* q = reinterpret_cast<const uint4*>(p - mis);
-    unpack_vec<T>(shifted(load16<RO>(q), load16<RO>(q + 1), mis * (int)sizeof(T)), v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; j++) v[j] = at + j >= 0 && at + j < V ? to_f32(p[j]) : -INFINITY;
-  }
-}
 template <typename T>
 DI uint4 pack_vec(const float* v) {
   uint32_t w[4];
@@ -284,6 +261,24 @@ DI uint4 pack_vec(const float* v) {
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The vector at entry `at` of a row that nothing writes meanwhile; what is past
+// the row's end is -inf.  Only 16-byte granules that lie in the row as a whole
+// are loaded as such: a row that starts `mis` entries into a granule takes two
+// of them.
+template <typename T>
+DI uint4 row_vec(const T* __restrict__ row, int at, int V, int mis) {
+  constexpr int VEC = Seg<T>::VEC;
+  const T* p = row + at;
+  if (mis == 0 && at + VEC <= V) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (mis != 0 && at >= mis && at - mis + 2 * VEC <= V) {
+    const uint4* q = reinterpret_cast<const uint4*>(p - mis);
+    return shifted(__ldg(q), __ldg(q + 1), mis * (int)sizeof(T));
+  }
+  float v[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; j++) v[j] = at + j < V ? to_f32(p[j]) : -INFINITY;
+  return pack_vec<T>(v);
 }
 template <typename T>
 DI int misaligned(const T* row) {
@@ -482,7 +477,7 @@ DI float segment_y(float ms, float m, float c) {
 // joins a row's segments (one warp; the result in every lane): at(i) gives
 // segment i's sums
 template <typename F>
-DI Sums join_segments(F at, int nseg, float c, float one) {
+DI Sums join_segments(F at, int nseg, float c, uint32_t table, float one) {
   const int l = threadIdx.x & 31;
   Sums t[kMaxSegs / 32];
   float m = -INFINITY;
@@ -497,7 +492,7 @@ DI Sums join_segments(F at, int nseg, float c, float one) {
   for (int i = 0; i < kMaxSegs / 32; i++) {
     if (32 * i >= nseg) break;
     const float y = segment_y(t[i].m, m, c);
-    const float f = exp2_one(y, one);
+    const float f = un(exp2_warp<true>(pk(y, y), table, pk(one, one)).e).x;
     s = fadd(s, fmul(f, t[i].s));
     // sum of 2^(y_j + y) (y_j + y) = f (w + y s); NaN stays NaN
     w = fadd(w, fmul(f, fadd(t[i].w, fmul(y, t[i].s))));
@@ -573,7 +568,8 @@ struct ListEntry {
 };
 // Thread i < k of the block gets entry i (blocks have at least DET_MAX_TOP
 // threads).  Begins and ends with the block in step.
-DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float c, float one, ListShared& sh) {
+DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float c, uint32_t table, float one,
+                           ListShared& sh) {
   const int t = threadIdx.x, w = t >> 5, l = t & 31, nw = blockDim.x >> 5;
   long long id = -1;
   float u = -INFINITY;
@@ -601,7 +597,7 @@ DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float c, float
     r.some |= sh.some[i] != 0;
   }
   r.d = valid ? fsub(u, m) : 0.0f;
-  const float e = valid ? exp2_one(fmul(r.d, c), one) : 0.0f;
+  const float y = fmul(r.d, c), p = un(exp2_warp<true>(pk(y, y), table, pk(one, one)).e).x, e = valid ? p : 0.0f;
   const float ws = warp_sum(e);
   if (l == 0) sh.sum[w] = ws;
   __syncthreads();
@@ -611,12 +607,16 @@ DI ListEntry teacher_entry(const Teacher& te, int row, int vocab, float c, float
   r.q = valid ? fdiv(e, r.s) : 0.0f;
   return r;
 }
+// log q of the thread's entry, in 64 bits
+DI double list_logq(const ListEntry& e, float temp) {
+  return e.id >= 0 ? dsub(ddiv((double)e.d, (double)temp), log_det((double)e.s)) : 0.0;
+}
 // the row's loss, in thread 0; z: the logit at the thread's entry.  Ends with
 // the block in step.
-DI float list_loss(const ListEntry& e, float z, const RowStats& r, double log_s, float temp, ListShared& sh) {
+DI float list_loss(const ListEntry& e, double logq, float z, const RowStats& r, double log_s, float temp,
+                   ListShared& sh) {
   double term = 0.0;
   if (e.id >= 0 && e.q > 0.0f) {
-    const double logq = dsub(ddiv((double)e.d, (double)temp), log_det((double)e.s));
     const double logp =
         r.empty ? (double)-INFINITY : dsub(ddiv(dsub((double)z, (double)r.m), (double)temp), log_s);
     term = dmul((double)e.q, dsub(logq, logp));
@@ -653,31 +653,31 @@ DI float list_share(ListEntry& e, int k, ListShared& sh) {
 // ---- the top list ------------------------------------------------------------------
 // The maximum of every group of adjacent entries is kept while a row's sums
 // are taken; the k largest entries lie in the groups whose maxima are among
-// the k largest, so only those are read again.  A group is what a warp loads
-// at once (128 f32 or 256 16-bit entries), or one lane's 16 bytes of it where
-// that would leave too few groups for a list (vocabularies up to 32,768).
-constexpr int kSmallVocab = 32768;
-constexpr int kCand = 2048;  // keys held before they are cut down to k
+// the k largest, so only those are read again.  A group is what 32, 8 or 1
+// lanes load at once (2^lg lanes of 16 bytes): the largest of them that leaves
+// 2 k groups, so that the entries above the k-th largest maximum are not many
+// more than k.  That is never more than kMaxGroups.
+constexpr int kRowThreads = DET_MAX_TOP;  // of a row's block: a thread per list entry
+constexpr int kMaxGroups = 2048;
+constexpr int kCand = 2304;               // keys held before they are cut down to k
+__host__ __device__ constexpr int group_lanes_log2(int V, int k, int vec) {
+  return V >= 2 * k * 32 * vec ? 5 : V >= 2 * k * 8 * vec ? 3 : 0;
+}
 struct TopShared {
-  unsigned long long key[kCand + kThreads];
-  int count, bits[2];
+  unsigned long long key[kCand];
+  int bin[256];
+  uint16_t group[kMaxGroups];
+  int count, groups, bits[3], floor_bin;
   uint32_t lo, hi;
 };
-template <typename T>
-DI int group_size(int V) {
-  return V <= kSmallVocab ? Seg<T>::VEC : Seg<T>::GROUP;
-}
-// A t that at least k of the block's values reach, and at most k + slack of
-// them where values are not equal (0 where there are fewer than k): bit by
-// bit below the bits that all of [lo, hi] share; lo <= every value <= hi.
-template <typename K, int PER>
-DI K kth_largest(const K (&v)[PER], K lo, K hi, int k, int slack, TopShared& sh) {
-  const K differ = lo ^ hi;
-  int bit = -1;
-  if (differ) bit = sizeof(K) == 8 ? 63 - __clzll((long long)differ) : 31 - __clz((int)differ);
-  K t = bit < 0 ? lo : lo & ~((K)2 * (((K)1 << bit) - 1) + 1);
-  for (int turn = 0; bit >= 0; bit--, turn ^= 1) {
-    const K cand = t | ((K)1 << bit);
+
+// The largest t that at least k of the block's values (distinct, or 0) reach,
+// bit by bit; done early once exactly k do.
+template <int PER>
+DI unsigned long long kth_largest(const unsigned long long (&v)[PER], int k, TopShared& sh) {
+  unsigned long long t = 0;
+  for (int bit = 63, turn = 0; bit >= 0; bit--) {
+    const unsigned long long cand = t | (1ull << bit);
     int c = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) c += v[i] >= cand;
@@ -685,13 +685,16 @@ DI K kth_largest(const K (&v)[PER], K lo, K hi, int k, int slack, TopShared& sh)
     if ((threadIdx.x & 31) == 0 && c) atomicAdd(&sh.bits[turn], c);
     __syncthreads();
     const int all = sh.bits[turn];
-    if (threadIdx.x == 0) sh.bits[turn ^ 1] = 0;
-    __syncthreads();
+    // the counter of the turn before: everyone has read it, and it is used
+    // again in two turns, behind another barrier
+    const int before = turn == 0 ? 2 : turn - 1;
+    if (threadIdx.x == 0) sh.bits[before] = 0;
+    turn = turn == 2 ? 0 : turn + 1;
     if (all >= k) t = cand;
-    if (all >= k && all <= k + slack) break;
+    if (all == k) break;
   }
   __syncthreads();
-  if (threadIdx.x == 0) sh.bits[0] = sh.bits[1] = 0;
+  if (threadIdx.x < 3) sh.bits[threadIdx.x] = 0;
   __syncthreads();
   return t;
 }
@@ -699,20 +702,17 @@ DI K kth_largest(const K (&v)[PER], K lo, K hi, int k, int slack, TopShared& sh)
 // smallest of them, or 0 if there are fewer than k
 DI unsigned long long cut_to(int k, TopShared& sh) {
   __syncthreads();
-  const int n = min(sh.count, kCand + kThreads);
-  if (n <= k) {
-    const unsigned long long r = 0;
-    __syncthreads();
-    return r;
-  }
-  constexpr int PER = (kCand + kThreads) / kThreads;
+  const int n = min(sh.count, kCand);
+  __syncthreads();
+  if (n <= k) return 0;
+  constexpr int PER = kCand / kRowThreads;
   unsigned long long v[PER];
 #pragma unroll
   for (int i = 0; i < PER; i++) {
-    const int at = i * kThreads + threadIdx.x;
+    const int at = i * kRowThreads + threadIdx.x;
     v[i] = at < n ? sh.key[at] : 0;
   }
-  const unsigned long long t = kth_largest<unsigned long long, PER>(v, 0ull, ~0ull, k, 0, sh);
+  const unsigned long long t = kth_largest<PER>(v, k, sh);
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
 #pragma unroll
@@ -721,101 +721,160 @@ DI unsigned long long cut_to(int k, TopShared& sh) {
   __syncthreads();
   return t;
 }
-// adds the entries of groups [g0, g1) whose keys are above `floor`
+// adds the entries of a vector whose keys are above `floor`
 template <typename T>
-DI void collect(const T* __restrict__ x, int V, int mis, const float* gmax, int g0, int g1, unsigned long long floor,
-                TopShared& sh) {
-  using G = Seg<T>;
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  auto push = [&](float v, int at) {
-    const unsigned long long key = top_key(v, (uint32_t)at);
-    if (at < V && key > floor) {
+DI void push_vec(uint4 w, int at, int V, unsigned long long floor, TopShared& sh) {
+  float v[Seg<T>::VEC];
+  unpack_vec<T>(w, v);
+#pragma unroll
+  for (int j = 0; j < Seg<T>::VEC; j++) {
+    const unsigned long long key = top_key(v[j], (uint32_t)(at + j));
+    if (at + j < V && key > floor) {
       const int slot = atomicAdd(&sh.count, 1);
-      if (slot < kCand + kThreads) sh.key[slot] = key;
-    }
-  };
-  if (V <= kSmallVocab) {
-    for (int g = g0 + threadIdx.x; g < g1; g += kThreads)
-      if (g * G::VEC < V && top_key(gmax[g], (uint32_t)(g * G::VEC)) > floor) {
-#pragma unroll
-        for (int j = 0; j < G::VEC; j++)
-          if (g * G::VEC + j < V) push(to_f32(x[g * G::VEC + j]), g * G::VEC + j);
-      }
-    return;
-  }
-  for (int b = g0 + 32 * w; b < g1; b += kThreads) {
-    const int mine = b + l;
-    const bool want =
-        mine < g1 && mine * G::GROUP < V && top_key(gmax[mine], (uint32_t)(mine * G::GROUP)) > floor;
-    for (unsigned todo = __ballot_sync(kFull, want); todo; todo &= todo - 1) {
-      const int at = (b + __ffs(todo) - 1) * G::GROUP + l * G::VEC;
-      float v[G::VEC];
-      load_vec<T>(x, at, V, mis, v);
-#pragma unroll
-      for (int j = 0; j < G::VEC; j++) push(v[j], at + j);
+      if (slot < kCand) sh.key[slot] = key;
     }
   }
 }
-template <int PER>
-DI unsigned long long list_floor(const float* gmax, int ng, int k, TopShared& sh) {
+// The row's k largest keys, in order, to sh.key[0 .. k); PER groups per thread
+// cover them all.  `meanwhile` runs while their maxima are on their way; the
+// list is not made where it gives false.
+template <typename T, int PER, typename F>
+DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int k, TopShared& sh, F meanwhile) {
+  constexpr int VEC = Seg<T>::VEC;
+  const int lg = group_lanes_log2(V, k, VEC), size = VEC << lg, ng = (V + size - 1) / size;
+  const int tid = threadIdx.x, l = tid & 31;
+  float f[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int g = i * kRowThreads + tid;
+    f[i] = g < ng ? gmax[g] : 0.0f;
+  }
+  if (!meanwhile()) return;
+  // the maxima, as ordered integers
   uint32_t v[PER], lo = ~0u, hi = 0;
 #pragma unroll
   for (int i = 0; i < PER; i++) {
-    const int g = i * kThreads + threadIdx.x;
-    const bool is = g < ng;
-    v[i] = is ? (uint32_t)(top_key(gmax[g], 0) >> 32) : 0u;
+    const int g = i * kRowThreads + tid;
+    v[i] = g < ng ? (uint32_t)(top_key(f[i], 0) >> 32) : 0u;
     hi = max(hi, v[i]);
-    if (is) lo = min(lo, v[i]);
+    if (g < ng) lo = min(lo, v[i]);
   }
+  if (tid == 0) sh.count = sh.groups = sh.bits[0] = sh.bits[1] = sh.bits[2] = 0, sh.lo = ~0u, sh.hi = 0;
+  for (int i = tid; i < 256; i += kRowThreads) sh.bin[i] = 0;
+  __syncthreads();
   hi = __reduce_max_sync(kFull, hi);
   lo = __reduce_min_sync(kFull, lo);
-  if ((threadIdx.x & 31) == 0) {
+  if (l == 0) {
     atomicMax(&sh.hi, hi);
     atomicMin(&sh.lo, lo);
   }
   __syncthreads();
-  const uint32_t t = kth_largest<uint32_t, PER>(v, sh.lo, sh.hi, k, k / 4 + 4, sh);
-  return t ? ((unsigned long long)t << 32) - 1 : 0;
-}
-// the row's k largest keys, in order, to sh.key[0 .. k)
-template <typename T>
-DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int k, TopShared& sh) {
-  const int ng = (V + group_size<T>(V) - 1) / group_size<T>(V);
-  if (threadIdx.x == 0) sh.count = sh.bits[0] = sh.bits[1] = 0, sh.lo = ~0u, sh.hi = 0;
-  __syncthreads();
-  // a value that at least k entries reach: about the k-th largest maximum
-  unsigned long long floor = 0;
+  // a value that at least k of them reach: the lower end of the bin, of 256
+  // between the smallest and the largest, that the k-th largest is in
+  uint32_t floor = 0;
   if (ng > k) {
-    floor = ng <= kThreads * 4   ? list_floor<4>(gmax, ng, k, sh)
-            : ng <= kThreads * 8 ? list_floor<8>(gmax, ng, k, sh)
-                                 : list_floor<kSmallVocab / 4 / kThreads>(gmax, ng, k, sh);
-  }
-  collect<T>(x, V, mis, gmax, 0, ng, floor, sh);
-  __syncthreads();
-  if (sh.count > kCand + kThreads) {
-    // too many entries reach it (ties, or a row in order): group by group in
-    // the order of their indices, cutting the list down as it fills, which
-    // raises the floor and passes over groups that cannot add to it
-    const int step = (kCand + kThreads - (int)DET_MAX_TOP) / group_size<T>(V);
+    lo = sh.lo;
+    const int shift = max(0, 24 - __clz((int)(sh.hi - lo)));
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (i * kRowThreads + tid < ng) atomicAdd(&sh.bin[(v[i] - lo) >> shift], 1);
     __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    for (int g = 0; g < ng; g += step) {
-      collect<T>(x, V, mis, gmax, g, min(ng, g + step), floor, sh);
-      const unsigned long long t = cut_to(k, sh);
-      if (t) floor = t;
+    if (tid < 32) {
+      int own = 0, c[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) own += c[i] = sh.bin[8 * l + i];
+      int above = own;  // of this lane's bins and those above
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_down_sync(kFull, above, o);
+        if (l + o < 32) above += t;
+      }
+      if (above >= k && above - own < k) {
+        int n = above - own, b = 7;
+        while ((n += c[b]) < k) b--;
+        sh.floor_bin = 8 * l + b;
+      }
     }
-  } else if (sh.count > kThreads) {
-    cut_to(k, sh);
+    __syncthreads();
+    floor = lo + ((uint32_t)sh.floor_bin << shift);
+  }
+  // the groups that reach it
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int g = i * kRowThreads + tid;
+    const bool in = g < ng && v[i] >= floor;
+    const unsigned who = __ballot_sync(kFull, in);
+    int base = 0;
+    if (l == 0 && who) base = atomicAdd(&sh.groups, __popc(who));
+    base = __shfl_sync(kFull, base, 0);
+    if (in) sh.group[base + __popc(who & ((1u << l) - 1))] = g;
   }
   __syncthreads();
-  // at most kThreads keys are left: each finds its rank
-  const int n = sh.count;
-  const unsigned long long mine = (int)threadIdx.x < n ? sh.key[threadIdx.x] : 0;
-  int rank = 0;
-  for (int i = 0; i < n; i++) rank += sh.key[i] > mine;
+  const int items = sh.groups << lg;
+  const bool few = sh.groups <= 4 * k + 64;
+  unsigned long long key_floor = floor ? ((unsigned long long)floor << 32) - 1 : 0;
+  if (few) {
+    // the usual case: their vectors, as many as can be on their way at once
+    constexpr int U = 8;
+    for (int j0 = tid; j0 < items; j0 += U * kRowThreads) {
+      uint4 w[U];
+      int at[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int j = j0 + u * kRowThreads;
+        at[u] = j < items ? ((sh.group[j >> lg] << lg) + (j & ((1 << lg) - 1))) * VEC : V;
+        if (at[u] < V) w[u] = row_vec<T>(x, at[u], V, mis);
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (at[u] < V) push_vec<T>(w[u], at[u], V, key_floor, sh);
+    }
+  }
   __syncthreads();
-  if ((int)threadIdx.x < n && rank < k) sh.key[rank] = mine;
+  if (!few || sh.count > kCand) {
+    // too many groups or entries reach the floor (ties, or a row in order): group by group in the order of their indices, cutting the list
+    // down as it fills, which raises the floor and passes over the groups that
+    // cannot add to it
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    const int step = max(1, (kCand - (int)DET_MAX_TOP) / size);
+    int g = 0;
+    while (g < ng) {
+      // as many groups as surely fit, of those that can add something
+      const int room = (kCand - sh.count) / size;
+      __syncthreads();
+      int g1 = g;
+      if (room > 0) {
+        g1 = min(ng, g + min(step, room));
+        for (int j = tid; j < (g1 - g) << lg; j += kRowThreads) {
+          const int q = g + (j >> lg), a = ((g << lg) + j) * VEC;
+          if (a < V && top_key(gmax[q], (uint32_t)(q * size)) > key_floor)
+            push_vec<T>(row_vec<T>(x, a, V, mis), a, V, key_floor, sh);
+        }
+      }
+      g = g1;
+      __syncthreads();
+      if (sh.count > kCand - size) {
+        const unsigned long long t = cut_to(k, sh);
+        if (t) key_floor = t;
+      }
+      __syncthreads();
+    }
+  }
+  if (sh.count > 2 * kRowThreads) cut_to(k, sh);
+  __syncthreads();
+  // at most two keys per thread are left: each finds its rank
+  const int n = sh.count, second = kRowThreads + tid;
+  const unsigned long long a = tid < n ? sh.key[tid] : 0, b = second < n ? sh.key[second] : 0;
+  int ra = 0, rb = 0;
+  for (int i = 0; i < n; i++) {
+    const unsigned long long o = sh.key[i];
+    ra += o > a;
+    rb += o > b;
+  }
+  __syncthreads();
+  if (a && ra < k) sh.key[ra] = a;
+  if (b && rb < k) sh.key[rb] = b;
   __syncthreads();
 }
 
@@ -838,7 +897,10 @@ DI uint32_t remote(const void* p, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   return r;
 }
-DI void store_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+DI void store_remote(uint32_t at, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
 
 // what a row's scores are written to (one thread)
 DI void write_stats(float* stats, int row, const RowStats& r, double log_s) {
@@ -869,8 +931,8 @@ struct Workspace {
   float4* seg;  // [rows][segments]: m, s, w
   float* gmax;  // [rows][groups]
 };
-enum : int { GROUPS_NONE, GROUPS_LANE, GROUPS_WARP };  // which maxima a top list needs
-template <typename T, int GROUPS>
+// LG: which maxima a top list needs, of 2^LG lanes' vectors; -1: none
+template <typename T, int LG>
 __global__ void __launch_bounds__(kSegThreads, kSegBlocks)
     segments_kernel(Logits L, float temp, Workspace ws, float one) {
   using G = Seg<T>;
@@ -895,22 +957,25 @@ __global__ void __launch_bounds__(kSegThreads, kSegBlocks)
     Range<T> all_range;
     float gm = -INFINITY;
     const size_t part = (size_t)row * nseg + g;
-    float* gmax = ws.gmax + part * (kSeg / G::VEC) + l;
+    float* gmax = ws.gmax + ((part * (kSeg / G::VEC)) >> (LG < 0 ? 0 : LG));
 #pragma unroll
     for (int i = 0; i < G::NV; i++) {
       all_range.take(v[i]);
-      if constexpr (GROUPS == GROUPS_NONE) continue;
-      Range<T> group;
-      group.take(v[i]);
-      const float lm = group.high();
-      if constexpr (GROUPS == GROUPS_LANE) gmax[i * 32] = lm;
-      if constexpr (GROUPS == GROUPS_WARP) {
-        const float r = redux_max(lm);
-        if (l == i) gm = r;
+      if constexpr (LG >= 0) {
+        Range<T> group;
+        group.take(v[i]);
+        float gh = group.high();
+        if constexpr (LG == 5) {
+          gh = redux_max(gh);
+          if (l == i) gm = gh;
+        } else {
+          for (int o = 1; o < 1 << LG; o <<= 1) gh = fmaxf(gh, __shfl_xor_sync(kFull, gh, o));
+          if ((l & ((1 << LG) - 1)) == 0) gmax[(i * 32 + l) >> LG] = gh;
+        }
       }
     }
-    if constexpr (GROUPS == GROUPS_WARP) {
-      if (l < G::NV) ws.gmax[part * G::NV + l] = gm;
+    if constexpr (LG == 5) {
+      if (l < G::NV) gmax[l] = gm;
     }
     const float m = redux_max(all_range.high()), low = redux_min(all_range.low());
     const float s = segment_sums<T, false>(v, V - g * kSeg, m, low, c, table, one, nullptr);
@@ -921,50 +986,53 @@ __global__ void __launch_bounds__(kSegThreads, kSegBlocks)
   }
 }
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(TOP ? kThreads : (int)DET_MAX_TOP)
+__global__ void __launch_bounds__(kRowThreads, 7)
     rows_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, Workspace ws, float* loss,
                 ScoreOut o, float one) {
   __shared__ ListShared list;
   const int row = blockIdx.x, V = L.vocab, nseg = (V + kSeg - 1) / kSeg;
   const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
   const float c = fdiv(kLog2e, temp), nan = __int_as_float(0x7fffffff);
+  const uint32_t table = kExpTable[threadIdx.x & 31];
   // what does not depend on the sums, while they are being taken
   ListEntry e;
   float z = 0.0f;
+  double logq = 0.0;
   long long t = -1;
   if (loss) {
-    e = teacher_entry(te, row, V, c, one, list);
+    e = teacher_entry(te, row, V, c, table, one, list);
     if (e.id >= 0) z = to_f32(x[e.id]);
+    logq = list_logq(e, temp);
   } else if (o.logprob) {
     t = load_id(tokens, id_bytes, row);
     if (t >= 0 && t < V) z = to_f32(x[t]);
   }
   pdl_wait();
-  const float4* seg = ws.seg + (size_t)row * nseg;
-  const RowStats r = finish_row(join_segments(
-      [&](int i) {
-        const float4 f = seg[i];
-        return Sums{f.x, f.y, f.z};
-      },
-      nseg, c, one));
-  const double log_s = log_sum(r);
-  if (threadIdx.x == 0) {
-    if (o.stats) write_stats(o.stats, row, r, log_s);
-    if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
-  }
-  if (loss) {
-    const float v = list_loss(e, z, r, log_s, temp, list);
+  RowStats r;
+  double log_s;
+  auto scores = [&]() {
+    const float4* seg = ws.seg + (size_t)row * nseg;
+    r = finish_row(join_segments(
+        [&](int i) {
+          const float4 f = seg[i];
+          return Sums{f.x, f.y, f.z};
+        },
+        nseg, c, table, one));
+    log_s = log_sum(r);
     if (threadIdx.x == 0) {
-      loss[row] = v;
-      if (e.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
+      if (o.stats) write_stats(o.stats, row, r, log_s);
+      if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+      if (!loss) write_scores(o, row, V, r, log_s, t, z);
+      if (t >= V && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
     }
-  } else if (threadIdx.x == 0) {
-    write_scores(o, row, V, r, log_s, t, z);
-    if (t >= V && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
-  }
+    return !r.bad;
+  };
   if constexpr (TOP) {
     __shared__ TopShared top;
-    if (!r.bad) top_list<T>(x, V, misaligned(x), ws.gmax + (size_t)row * nseg * (kSeg / group_size<T>(V)), o.top, top);
+    const int lg = group_lanes_log2(V, o.top, Seg<T>::VEC);
+    const float* gmax = ws.gmax + (((size_t)row * nseg * (kSeg / Seg<T>::VEC)) >> lg);
+    if (V <= (Seg<T>::VEC << lg) * 8 * kRowThreads) top_list<T, 8>(x, V, misaligned(x), gmax, o.top, top, scores);
+    else top_list<T, kMaxGroups / kRowThreads>(x, V, misaligned(x), gmax, o.top, top, scores);
     if ((int)threadIdx.x < o.top) {
       const size_t at = (size_t)row * o.top + threadIdx.x;
       const unsigned long long key = r.bad ? 0 : top.key[threadIdx.x];
@@ -973,6 +1041,15 @@ __global__ void __launch_bounds__(TOP ? kThreads : (int)DET_MAX_TOP)
         o.top_logprobs[at] = r.bad     ? nan
                              : r.empty ? -INFINITY
                                        : (float)dsub(dsub((double)key_value(key), (double)r.m), log_s);
+      }
+    }
+  } else {
+    scores();
+    if (loss) {
+      const float v = list_loss(e, logq, z, r, log_s, temp, list);
+      if (threadIdx.x == 0) {
+        loss[row] = v;
+        if (e.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
       }
     }
   }
@@ -1070,7 +1147,7 @@ __global__ void __launch_bounds__(kThreads, 3)
   int id;
   float add;
   if (te.k) {
-    ListEntry e = teacher_entry(te, row, V, c, one_, sh);
+    ListEntry e = teacher_entry(te, row, V, c, table, one_, sh);
     const float g_t = fdiv(in.g[row], temp);
     r = list_grad(e, g_t, m, s, c);
     add = fmul(-g_t, list_share(e, te.k, sh));
@@ -1186,19 +1263,62 @@ DI void store_segment(T* y, int g, int V, int my, F vec) {
   }
 }
 
-// Clusters take rows in turn; each of a cluster's warps holds one segment of
-// the row, so the row is read once: its exponentials stay in registers until
-// every block has all segments' sums, and are scaled and stored then, while
-// the next row's segment is on its way.  The entropy's gradient needs y too:
-// it keeps the logits and takes their exponentials again.
+// Three kernels.  The first gathers what the gradient's coefficients and the
+// logits at a row's own tokens are, before `out` may overwrite those.  In the
+// second, clusters take rows in turn; each of a cluster's warps holds one
+// segment of the row, so the row is read once: its exponentials stay in
+// registers until every block has all segments' sums, and are scaled and
+// stored then, while the next row's segment is on its way.  (The entropy's
+// gradient needs y too: it keeps the logits and takes their exponentials
+// again.)  One cluster barrier per row: the sums have two places, and a warp
+// writes to one of them again only behind the barrier of the row between, at
+// which every warp has read it.  The third writes the rows' scores and adds
+// the part of their own tokens.
+struct StepWork {
+  float4* coef;  // per row: of the loss over T, or of logprob; of the entropy; 1 where there is nothing but zeros
+  float* z;      // per row and entry: the logit at its token
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    step_gather_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, StepWork ws) {
+  pdl_trigger();
+  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), l = threadIdx.x & 31, V = L.vocab;
+  if (row >= L.n) return;
+  const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
+  const float nan = __int_as_float(0x7fffffff);
+  if (te.k) {
+    bool some = false, bad = false;
+    for (int i = l; i < te.k; i += 32) {
+      const long long id = load_id(te.ids, te.id_bytes, (size_t)row * te.ld + i);
+      if (id < 0) continue;
+      const float u = load_any(te.u, te.dtype, (size_t)row * te.ld + i);
+      bad |= id >= V || !(u < INFINITY);
+      some |= u > -INFINITY;
+      if (id < V) ws.z[(size_t)row * te.k + i] = to_f32(x[id]);
+    }
+    some = __any_sync(kFull, some);
+    bad = __any_sync(kFull, bad);
+    if (l == 0)
+      ws.coef[row] = make_float4(bad ? nan : fdiv(in.g[row], temp), 0.0f, !some && !bad ? 1.0f : 0.0f, 0.0f);
+  } else if (l == 0) {
+    const long long t = tokens ? load_id(tokens, id_bytes, row) : -1;
+    if (t >= 0 && t < V) ws.z[row] = to_f32(x[t]);
+    const float gl = !in.g || t < 0 ? 0.0f : t >= V ? nan : in.g[row];
+    ws.coef[row] = make_float4(-gl, in.gh ? in.gh[row] : 0.0f, 0.0f, 0.0f);
+  }
+}
+// the coefficients of a row: a_g, a_h as in StepWork, of the loss over T or of
+// minus the logprob, and of the entropy
+DI RowGrad row_grad(float a_g, float a_h, bool zero, const RowStats& r, float c) {
+  const float inv_s = fdiv(1.0f, r.s);
+  const float a = a_h == 0.0f ? a_g : fadd(a_g, fmul(a_h, fdiv(r.s1, r.s)));
+  return {-r.m, c, fmul(a, inv_s), fmul(fmul(-a_h, kLn2), inv_s), zero || r.empty};
+}
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, 2)
-    step_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, float* loss,
-                ScoreOut o, T* out, unsigned long long out_ld, float one_) {
-  __shared__ struct {
-    float m[kMaxSegs], s[kMaxSegs], w[kMaxSegs];
-    ListShared list;
-  } sh;
+    step_kernel(Logits L, float temp, StepWork ws, float* stats, T* out, unsigned long long out_ld, float one_) {
+  using G = Seg<T>;
+  __shared__ float4 seg[2][kMaxSegs];
   extern __shared__ __align__(16) uint8_t dyn[];
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -1209,50 +1329,33 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto at_row = [&](int r) { return static_cast<const T*>(L.x) + (size_t)r * L.ld; };
   int row = blockIdx.x / size;
   if (row < L.n && active) stage_issue<T>(stage, at_row(row), g, V);
+  pdl_trigger();
   const float c = fdiv(kLog2e, temp);
   const uint32_t table = kExpTable[l];
-  if (size > 1) cluster_arrive();
-  for (; row < L.n; row += clusters) {
-    const T* x = at_row(row);
-    T* y = out + (size_t)row * out_ld;
-    uint4 raw[Seg<T>::NV];
+  const uint32_t place = remote(&seg[0][g < kMaxSegs ? g : 0], l < (int)size ? l : 0);
+  if (size > 1) {  // every block runs before anyone writes to it
+    cluster_arrive();
+    cluster_wait();
+  }
+  bool gathered = false;
+  float4 coef;
+  for (int turn = 0; row < L.n; row += clusters, turn ^= 1) {
+    uint4 raw[G::NV];
     float v[ENTROPY ? 1 : kPerLane];
+    if (gathered) coef = ws.coef[row];
     float m_seg = -INFINITY, s_seg = 0.0f, w_seg = 0.0f;
     if (active) {
-      stage_take<T>(stage, misaligned(x), raw);
+      stage_take<T>(stage, misaligned(at_row(row)), raw);
       if (row + clusters < L.n) stage_issue<T>(stage, at_row(row + clusters), g, V);
       Range<T> range;
 #pragma unroll
-      for (int i = 0; i < Seg<T>::NV; i++) range.take(raw[i]);
+      for (int i = 0; i < G::NV; i++) range.take(raw[i]);
       m_seg = redux_max(range.high());
       s_seg = segment_sums<T, !ENTROPY>(raw, V - g * kSeg, m_seg, redux_min(range.low()), c, table, one_, v);
       w_seg = __shfl_sync(kFull, s_seg, 16);
       s_seg = __shfl_sync(kFull, s_seg, 0);
-    }
-    // the row's own tokens, before `out` may overwrite their logits
-    ListEntry e;
-    long long t = -1;
-    int id;
-    float share = 0.0f;
-    if (te.k) {
-      e = teacher_entry(te, row, V, c, one_, sh.list);
-      id = e.id;
-    } else {
-      t = tokens ? load_id(tokens, id_bytes, row) : -1;
-      id = threadIdx.x == 0 && t >= 0 && t < V ? (int)t : -1;
-    }
-    const float z = id >= 0 ? to_f32(x[id]) : 0.0f;
-    if (te.k) {
-      ListEntry f = e;
-      share = list_share(f, te.k, sh.list);
-      id = f.id;
-    }
-    if (size > 1) cluster_wait();
-    else __syncthreads();
-    if (active && l < (int)size) {
-      store_remote(remote(&sh.m[g], l), m_seg);
-      store_remote(remote(&sh.s[g], l), s_seg);
-      store_remote(remote(&sh.w[g], l), w_seg);
+      if (l < (int)size)
+        store_remote(place + turn * (uint32_t)sizeof(seg[0]), make_float4(m_seg, s_seg, w_seg, 0.0f));
     }
     if (size > 1) {
       cluster_arrive();
@@ -1260,24 +1363,30 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else {
       __syncthreads();
     }
-    const RowStats r =
-        finish_row(join_segments([&](int i) { return Sums{sh.m[i], sh.s[i], sh.w[i]}; }, nseg, c, one_));
-    if (size > 1) cluster_arrive();
-    RowGrad rg;
-    float add;
-    if (te.k) {
-      const float g_t = fdiv(in.g[row], temp);
-      rg = list_grad(e, g_t, r.m, r.s, c);
-      add = fmul(-g_t, share);
-    } else {
-      rg = score_grad(in, row, V, t, r.m, r.s, r.s1, c, &add);
+    if (!gathered) {  // the first kernel's results, and its reads are done
+      pdl_wait();
+      gathered = true;
+      coef = ws.coef[row];
+    }
+    const RowStats r = finish_row(join_segments(
+        [&](int i) {
+          const float4 f = seg[turn][i];
+          return Sums{f.x, f.y, f.z};
+        },
+        nseg, c, table, one_));
+    const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
+    if (rank == 0 && threadIdx.x == 0) {
+      float* st = stats + (size_t)row * 4;
+      st[0] = r.m, st[1] = r.s, st[2] = r.s1;
     }
     if (active) {
       const f2 one = pk(one_, one_), cc = pk(c, c);
-      const float f = fmul(exp2_one(segment_y(m_seg, r.m, c), one_), rg.as);
+      const float y_seg = segment_y(m_seg, r.m, c);
+      const float f = fmul(un(exp2_warp<true>(pk(y_seg, y_seg), table, one).e).x, rg.as);
       // vector i of the segment's gradient
       auto vec = [&](int i) {
-        constexpr int VEC = Seg<T>::VEC;
+        constexpr int VEC = G::VEC;
+        if (rg.zero) return make_uint4(0, 0, 0, 0);
         float x[VEC];
         f2 dx[VEC / 2];
         if constexpr (ENTROPY) add_vec<T>(raw[i], rg.base, dx);
@@ -1291,31 +1400,67 @@ __global__ void __launch_bounds__(kThreads, 2)
             d = mul2(pk(v[i * VEC + j], v[i * VEC + j + 1]), pk(f, f));
           }
           const float2 dv = un(d);
-          x[j] = rg.zero ? 0.0f : dv.x;
-          x[j + 1] = rg.zero ? 0.0f : dv.y;
+          x[j] = dv.x;
+          x[j + 1] = dv.y;
         }
         return pack_vec<T>(x);
       };
+      T* y = out + (size_t)row * out_ld;
       store_segment<T>(y, g, V, misaligned(y), vec);
     }
-    if (rank == 0) {
-      const double log_s = log_sum(r);
-      if (threadIdx.x == 0) {
-        if (o.stats) write_stats(o.stats, row, r, log_s);
-        if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
-        if ((te.k ? e.bad : t >= V) && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
-        if (!te.k) write_scores(o, row, V, r, log_s, t, z);
-      }
-      if (te.k) {
-        const float lv = list_loss(e, z, r, log_s, temp, sh.list);
-        if (threadIdx.x == 0) loss[row] = lv;
-      }
-    }
-    __syncthreads();  // the segments are stored
-    if (id >= (int)rank * warps * kSeg && id < (int)(rank + 1) * warps * kSeg && !rg.zero)
-      y[id] = from_f32<T>(fadd(grad1<ENTROPY>(z, rg, one_), add));
   }
-  if (size > 1) cluster_wait();
+  if (size > 1) {  // nobody leaves while another block may still write to it
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kRowThreads)
+    step_rows_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, StepWork ws,
+                     float* loss, ScoreOut o, T* out, unsigned long long out_ld, float one) {
+  __shared__ ListShared list;
+  const int row = blockIdx.x, V = L.vocab;
+  const float c = fdiv(kLog2e, temp);
+  const uint32_t table = kExpTable[threadIdx.x & 31];
+  ListEntry e;
+  double logq = 0.0;
+  long long t = -1;
+  int id, own;
+  float share = 0.0f;
+  if (loss) {
+    e = teacher_entry(te, row, V, c, table, one, list);
+    logq = list_logq(e, temp);
+    own = e.id;
+    ListEntry f = e;
+    share = list_share(f, te.k, list);
+    id = f.id;
+  } else {
+    t = tokens ? load_id(tokens, id_bytes, row) : -1;
+    own = id = threadIdx.x == 0 && t >= 0 && t < V ? (int)t : -1;
+  }
+  pdl_wait();
+  const float z = own >= 0 ? ws.z[(size_t)row * (loss ? te.k : 1) + threadIdx.x] : 0.0f;
+  const float4 coef = ws.coef[row];
+  const float* st = o.stats + (size_t)row * 4;
+  RowStats r;
+  r.m = st[0], r.s = st[1], r.s1 = st[2];
+  r.bad = !(r.m == r.m), r.empty = r.m == -INFINITY;
+  const double log_s = log_sum(r);
+  const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
+  if (id >= 0 && !rg.zero) {
+    const float add = loss ? fmul(-coef.x, share) : -coef.x;
+    out[(size_t)row * out_ld + id] = from_f32<T>(fadd(grad1<ENTROPY>(z, rg, one), add));
+  }
+  if (threadIdx.x == 0) {
+    o.stats[(size_t)row * 4 + 3] = (float)log_s;
+    if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+    if ((loss ? e.bad : t >= V) && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
+    if (!loss) write_scores(o, row, V, r, log_s, t, z);
+  }
+  if (loss) {
+    const float v = list_loss(e, logq, z, r, log_s, temp, list);
+    if (threadIdx.x == 0) loss[row] = v;
+  }
 }
 
 // ---- launches --------------------------------------------------------------------
@@ -1355,7 +1500,8 @@ int resident_clusters(const void* kern, int c, int threads, size_t smem) {
   }
   return n = got;
 }
-// launches `clusters` clusters of c blocks
+// launches `clusters` clusters of c blocks, with programmatic stream
+// serialization
 template <typename... KArgs, typename... Args>
 cudaError_t launch_clusters(cudaStream_t s, void (*kern)(KArgs...), int clusters, int c, int threads, size_t smem,
                             Args... args) {
@@ -1364,12 +1510,14 @@ cudaError_t launch_clusters(cudaStream_t s, void (*kern)(KArgs...), int clusters
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = c;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = c > 1;
+  cfg.numAttrs = c > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 // clusters above 8 blocks have to be allowed, once per kernel and device
@@ -1389,15 +1537,17 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // what a forward call keeps between its two kernels
 size_t workspace_bytes(int dtype, int n, int vocab, int top) {
   const size_t nseg = (vocab + kSeg - 1) / kSeg, vec = dtype == DET_DTYPE_F32 ? 4 : 8;
-  const size_t groups = !top ? 0 : nseg * kSeg / (vocab <= kSmallVocab ? vec : 32 * vec);
+  const size_t groups = !top ? 0 : nseg * kSeg / (vec << group_lanes_log2(vocab, top, (int)vec));
   return align256(n * nseg * sizeof(float4)) + align256(n * groups * sizeof(float));
 }
 template <typename T, bool TOP>
 cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te,
                        float temp, void* workspace, float* loss, const ScoreOut& o) {
-  const auto segments = !TOP                       ? segments_kernel<T, GROUPS_NONE>
-                        : L.vocab <= kSmallVocab ? segments_kernel<T, GROUPS_LANE>
-                                                 : segments_kernel<T, GROUPS_WARP>;
+  const int lg = TOP ? group_lanes_log2(L.vocab, o.top, Seg<T>::VEC) : -1;
+  const auto segments = lg < 0    ? segments_kernel<T, -1>
+                        : lg == 0 ? segments_kernel<T, 0>
+                        : lg == 3 ? segments_kernel<T, 3>
+                                  : segments_kernel<T, 5>;
   constexpr int kSegWarps = kSegThreads / 32;
   const size_t smem = kSegWarps * kStageBytes<T>;
   if (cudaError_t e = raise_smem_cap((const void*)segments, smem)) return e;
@@ -1409,7 +1559,7 @@ cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int 
   segments<<<(unsigned)(blocks < fit ? blocks : fit), kSegThreads, smem, s>>>(L, temp, ws, 1.0f);
   if (cudaError_t e = cudaGetLastError()) return e;
   const Launch launch{s, nullptr, nullptr, true};
-  return launch_k(launch, rows_kernel<T, TOP>, dim3(L.n), dim3(TOP ? kThreads : DET_MAX_TOP), 0, L, tokens, id_bytes,
+  return launch_k(launch, rows_kernel<T, TOP>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes,
                   te, temp, ws, loss, o, 1.0f);
 }
 cudaError_t launch_forward(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
@@ -1448,28 +1598,38 @@ cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* 
   });
 }
 
+size_t step_workspace_bytes(size_t n, int k) { return align256(n * sizeof(float4)) + align256(n * k * sizeof(float)); }
 template <typename T, bool ENTROPY>
 cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
-                    const GradIn& in, float* loss, const ScoreOut& o, void* out, unsigned long long out_ld) {
+                    const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
+                    unsigned long long out_ld) {
+  const StepWork ws{static_cast<float4*>(workspace),
+                    reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256(L.n * sizeof(float4)))};
   const auto kern = step_kernel<T, ENTROPY>;
-  // a warp per segment; at least DET_MAX_TOP threads, one per list entry
-  const int nseg = (L.vocab + kSeg - 1) / kSeg, c = (nseg + kWarps - 1) / kWarps;
-  const int need = (nseg + c - 1) / c, warps = need < (int)DET_MAX_TOP / 32 ? (int)DET_MAX_TOP / 32 : need;
+  // a warp per segment
+  const int nseg = (L.vocab + kSeg - 1) / kSeg, c = (nseg + kWarps - 1) / kWarps, warps = (nseg + c - 1) / c;
   const size_t smem = warps * kStageBytes<T>;
   if (cudaError_t e = raise_smem_cap((const void*)kern, smem)) return e;
   if (c > 8)
     if (cudaError_t e = allow_large_clusters((const void*)kern)) return e;
   const int fit = resident_clusters((const void*)kern, c, 32 * warps, smem);
-  return launch_clusters(s, kern, L.n < fit ? L.n : fit, c, 32 * warps, smem, L, tokens, id_bytes, te, temp, in, loss,
-                         o, static_cast<T*>(out), out_ld, 1.0f);
+  step_gather_kernel<T><<<(L.n + kWarps - 1) / kWarps, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, ws);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  T* y = static_cast<T*>(out);
+  if (cudaError_t e = launch_clusters(s, kern, L.n < fit ? L.n : fit, c, 32 * warps, smem, L, temp, ws, o.stats, y,
+                                      out_ld, 1.0f))
+    return e;
+  const Launch launch{s, nullptr, nullptr, true};
+  return launch_k(launch, step_rows_kernel<T, ENTROPY>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes, te, temp,
+                  in, ws, loss, o, y, out_ld, 1.0f);
 }
 cudaError_t launch_step(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
-                        const Teacher& te, float temp, const GradIn& in, float* loss, const ScoreOut& o, void* out,
-                        unsigned long long out_ld) {
+                        const Teacher& te, float temp, const GradIn& in, void* workspace, float* loss,
+                        const ScoreOut& o, void* out, unsigned long long out_ld) {
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    return in.gh ? step_as<T, true>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld)
-                 : step_as<T, false>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld);
+    return in.gh ? step_as<T, true>(s, L, tokens, id_bytes, te, temp, in, workspace, loss, o, out, out_ld)
+                 : step_as<T, false>(s, L, tokens, id_bytes, te, temp, in, workspace, loss, o, out, out_ld);
   });
 }
 
@@ -1513,10 +1673,8 @@ det_status check_list(const void* ids, int id_bytes, const void* teacher, int te
   if (!(temperature >= DET_MIN_TEMPERATURE && temperature <= DET_MAX_TEMPERATURE)) return DET_ERR_INVALID_ARGUMENT;
   return DET_OK;
 }
-det_status check_workspace(const void* workspace, size_t size, int dtype, uint32_t n, uint32_t vocab, uint32_t top) {
-  if (!workspace || (uintptr_t)workspace % 16 || size < workspace_bytes(dtype, (int)n, (int)vocab, (int)top))
-    return DET_ERR_INVALID_ARGUMENT;
-  return DET_OK;
+det_status check_workspace(const void* workspace, size_t size, size_t need) {
+  return workspace && (uintptr_t)workspace % 16 == 0 && size >= need ? DET_OK : DET_ERR_INVALID_ARGUMENT;
 }
 det_status check_device() {
   int cnt = 0;
@@ -1563,6 +1721,10 @@ size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top)
   return workspace_bytes(dtype, (int)n, (int)vocab, (int)top);
 }
 
+size_t det_step_workspace(uint32_t n, uint32_t k) {
+  return n > DET_SCORE_MAX_ROWS || k > DET_MAX_TOP ? 0 : step_workspace_bytes(n, k ? (int)k : 1);
+}
+
 det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* tokens, int token_bytes, uint32_t top, float* logprob, float* entropy,
                                    float* stats, int32_t* top_ids, float* top_logprobs, uint32_t* flags,
@@ -1572,7 +1734,7 @@ det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, ui
   if (logprob)
     if (det_status st = check_ids(tokens, token_bytes)) return st;
   if (top > DET_MAX_TOP || top > vocab || (top && !top_ids && !top_logprobs)) return DET_ERR_INVALID_ARGUMENT;
-  if (det_status st = check_workspace(workspace, workspace_size, dtype, n, vocab, top)) return st;
+  if (det_status st = check_workspace(workspace, workspace_size, workspace_bytes(dtype, (int)n, (int)vocab, (int)top))) return st;
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const ScoreOut o{logprob, entropy, stats, top_ids, top_logprobs, (int)top, flags};
@@ -1599,19 +1761,21 @@ det_status det_token_scores_grad_device(const void* logits, int dtype, uint32_t 
 det_status det_token_scores_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                         const void* tokens, int token_bytes, const float* grad_logprob,
                                         const float* grad_entropy, float* logprob, float* entropy, float* stats,
-                                        void* grad, uint64_t grad_ld, uint32_t* flags, void* stream) {
+                                        void* grad, uint64_t grad_ld, uint32_t* flags, void* workspace,
+                                        size_t workspace_size, void* stream) {
   if (n == 0) return DET_OK;
   if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
   if (det_status st = check_grad(logits, dtype, n, vocab, ld, grad, grad_ld)) return st;
   if (!stats || (!grad_logprob && !grad_entropy)) return DET_ERR_INVALID_ARGUMENT;
   if (logprob || grad_logprob)
     if (det_status st = check_ids(tokens, token_bytes)) return st;
+  if (det_status st = check_workspace(workspace, workspace_size, step_workspace_bytes(n, 1))) return st;
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const ScoreOut o{logprob, entropy, stats, nullptr, nullptr, 0, flags};
   return launched(launch_step(static_cast<cudaStream_t>(stream), dtype, L, logprob || grad_logprob ? tokens : nullptr,
-                              token_bytes, kNoTeacher, 1.0f, GradIn{nullptr, grad_logprob, grad_entropy}, nullptr, o,
-                              grad, grad_ld));
+                              token_bytes, kNoTeacher, 1.0f, GradIn{nullptr, grad_logprob, grad_entropy}, workspace,
+                              nullptr, o, grad, grad_ld));
 }
 
 det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
@@ -1622,7 +1786,7 @@ det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, ui
   if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
   if (det_status st = check_list(ids, id_bytes, teacher, teacher_dtype, k, n, list_ld, temperature)) return st;
   if (!loss) return DET_ERR_INVALID_ARGUMENT;
-  if (det_status st = check_workspace(workspace, workspace_size, dtype, n, vocab, 0)) return st;
+  if (det_status st = check_workspace(workspace, workspace_size, workspace_bytes(dtype, (int)n, (int)vocab, 0))) return st;
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
@@ -1650,18 +1814,20 @@ det_status det_distill_grad_device(const void* logits, int dtype, uint32_t n, ui
 det_status det_distill_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
                                    uint64_t list_ld, float temperature, const float* grad_loss, float* loss,
-                                   float* stats, void* grad, uint64_t grad_ld, uint32_t* flags, void* stream) {
+                                   float* stats, void* grad, uint64_t grad_ld, uint32_t* flags, void* workspace,
+                                   size_t workspace_size, void* stream) {
   if (n == 0) return DET_OK;
   if (det_status st = check_logits(logits, dtype, n, vocab, ld)) return st;
   if (det_status st = check_grad(logits, dtype, n, vocab, ld, grad, grad_ld)) return st;
   if (det_status st = check_list(ids, id_bytes, teacher, teacher_dtype, k, n, list_ld, temperature)) return st;
   if (!loss || !stats || !grad_loss) return DET_ERR_INVALID_ARGUMENT;
+  if (det_status st = check_workspace(workspace, workspace_size, step_workspace_bytes(n, (int)k))) return st;
   if (det_status st = check_device()) return st;
   const Logits L{logits, nullptr, ld, (int)n, (int)vocab};
   const Teacher te{ids, teacher, list_ld, id_bytes, teacher_dtype, (int)k};
   const ScoreOut o{nullptr, nullptr, stats, nullptr, nullptr, 0, flags};
   return launched(launch_step(static_cast<cudaStream_t>(stream), dtype, L, nullptr, 4, te, temperature,
-                              GradIn{nullptr, grad_loss, nullptr}, loss, o, grad, grad_ld));
+                              GradIn{nullptr, grad_loss, nullptr}, workspace, loss, o, grad, grad_ld));
 }
 
 }  // extern "C"

@@ -977,7 +977,7 @@ static constexpr size_t kScoreBytes = (size_t)kScoreRows * (16 + 8 * DET_MAX_TOP
 static det_status score_buffers(det_session* s) {
   const int rows = std::min<int>(s->max_chunk, kScoreRows);
   if (!s->d_score)
-    if (det_status st = dalloc(s, &s->d_score, kScoreBytes + scores_workspace_bytes(rows, s->m->vocab, 1))) return st;
+    if (det_status st = dalloc(s, &s->d_score, kScoreBytes + scores_workspace_bytes(rows, s->m->vocab, DET_MAX_TOP))) return st;
   return s->h_score ? DET_OK : halloc(s, &s->h_score, kScoreBytes);
 }
 

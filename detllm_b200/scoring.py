@@ -107,8 +107,7 @@ def _new(logits, *shape):
     return torch.empty(shape, dtype=torch.float32, device=logits.device)
 
 
-def _workspace(logits, n, vocab, top):
-    size = lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, top)
+def _workspace(logits, size):
     return torch.empty(size, dtype=torch.uint8, device=logits.device), size
 
 
@@ -125,7 +124,7 @@ def token_scores(logits, tokens, top: int = 0) -> TokenScores:
             raise ValueError("top must not be negative")
         ids = torch.empty((n, top), dtype=torch.int32, device=logits.device)
         lps = _new(logits, n, top)
-    work, size = _workspace(logits, n, vocab, top)
+    work, size = _workspace(logits, lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, top))
     _call("det_token_scores_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
           _IDS[tokens.dtype], top, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
           ids.data_ptr() if top else None, lps.data_ptr() if top else None, None, work.data_ptr(), size)
@@ -157,9 +156,10 @@ def token_scores_step(logits, tokens, grad_logprob=None, grad_entropy=None, out=
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     logprob, entropy, stats = _new(logits, n), _new(logits, n), _new(logits, n, 4)
+    work, size = _workspace(logits, lib().det_step_workspace(n, 1))
     _call("det_token_scores_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
           _IDS[tokens.dtype], gl, ge, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld,
-          None)
+          None, work.data_ptr(), size)
     return TokenScores(logprob, entropy, stats), out
 
 
@@ -171,7 +171,7 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) 
     n, vocab, ld = _logits(logits)
     lists = _lists(teacher_ids, teacher_logits, logits, n)
     loss, stats = _new(logits, n), _new(logits, n, 4)
-    work, size = _workspace(logits, n, vocab, 0)
+    work, size = _workspace(logits, lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, 0))
     _call("det_distill_loss_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
           temperature, loss.data_ptr(), stats.data_ptr(), None, work.data_ptr(), size)
     return DistillLoss(loss, stats)
@@ -200,6 +200,7 @@ def distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperature: fl
     g = _vector(grad_loss, logits, "grad_loss", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     loss, stats = _new(logits, n), _new(logits, n, 4)
+    work, size = _workspace(logits, lib().det_step_workspace(n, lists[4]))
     _call("det_distill_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
-          temperature, g, loss.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld, None)
+          temperature, g, loss.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld, None, work.data_ptr(), size)
     return DistillLoss(loss, stats), out

@@ -361,10 +361,12 @@ det_status det_token_scores(det_session* s, const uint32_t* rows, const uint32_t
                             float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs);
 det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, const uint32_t* teacher_ids,
                             const float* teacher_logits, uint32_t k, float temperature, float* loss);
-/* bytes of workspace that det_token_scores_device (and, with top = 0,
- * det_distill_loss_device) needs; 16-byte aligned.  Calls that may overlap
- * need one each; what it holds between calls does not matter. */
+/* Bytes of workspace that det_token_scores_device (and, with top = 0,
+ * det_distill_loss_device) needs, and that the step calls do (k entries per
+ * list, 1 for scores); 16-byte aligned.  Calls that may overlap need one each;
+ * what it holds between calls does not matter. */
 size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top);
+size_t det_step_workspace(uint32_t n, uint32_t k);
 /* log probability of tokens[i], entropy, and the `top` (<= DET_MAX_TOP, <=
  * vocab) most likely tokens of row i with their log probabilities, most
  * likely first, equal ones in the order of their ids: n x top each */
@@ -382,7 +384,8 @@ det_status det_token_scores_grad_device(const void* logits, int dtype, uint32_t 
 det_status det_token_scores_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                         const void* tokens, int token_bytes, const float* grad_logprob,
                                         const float* grad_entropy, float* logprob, float* entropy, float* stats,
-                                        void* grad, uint64_t grad_ld, uint32_t* flags, void* stream);
+                                        void* grad, uint64_t grad_ld, uint32_t* flags, void* workspace,
+                                        size_t workspace_size, void* stream);
 /* loss[i] of row i against the k (1 .. DET_MAX_TOP) entries of list i, at
  * temperature T (DET_MIN_TEMPERATURE .. DET_MAX_TEMPERATURE) on both sides */
 det_status det_distill_loss_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
@@ -398,7 +401,8 @@ det_status det_distill_grad_device(const void* logits, int dtype, uint32_t n, ui
 det_status det_distill_step_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,
                                    const void* ids, int id_bytes, const void* teacher, int teacher_dtype, uint32_t k,
                                    uint64_t list_ld, float temperature, const float* grad_loss, float* loss,
-                                   float* stats, void* grad, uint64_t grad_ld, uint32_t* flags, void* stream);
+                                   float* stats, void* grad, uint64_t grad_ld, uint32_t* flags, void* workspace,
+                                   size_t workspace_size, void* stream);
 
 #ifdef __cplusplus
 }

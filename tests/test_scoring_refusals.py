@@ -29,8 +29,9 @@ def scores_grad(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, tok=P, tb=8, st=P
 
 
 def scores_step(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, tok=P, tb=8, gl=P, ge=None, lp=P, en=P, st=P, out=P,
-                old=1000):
-    return lib.det_token_scores_step_device(x, dtype, n, vocab, ld, tok, tb, gl, ge, lp, en, st, out, old, None, None)
+                old=1000, ws=P, size=1 << 40):
+    return lib.det_token_scores_step_device(x, dtype, n, vocab, ld, tok, tb, gl, ge, lp, en, st, out, old, None, ws,
+                                            size, None)
 
 
 def loss(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, ids=P, ib=4, u=P, ud=F32, k=8, lld=8, t=1.0, out=P, st=P,
@@ -45,9 +46,9 @@ def loss_grad(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, ids=P, ib=4, u=P, u
 
 
 def loss_step(lib, x=P, dtype=F32, n=4, vocab=1000, ld=1000, ids=P, ib=4, u=P, ud=F32, k=8, lld=8, t=1.0, g=P, lo=P,
-              st=P, out=P, old=1000):
+              st=P, out=P, old=1000, ws=P, size=1 << 40):
     return lib.det_distill_step_device(x, dtype, n, vocab, ld, ids, ib, u, ud, k, lld, t, g, lo, st, out, old, None,
-                                       None)
+                                       ws, size, None)
 
 
 ALL = [scores, scores_grad, scores_step, loss, loss_grad, loss_step]
@@ -108,6 +109,17 @@ def test_workspace(lib, call):
     assert lib.det_scores_workspace(F32, 4, 1000, 5) > need  # a top list keeps more
     assert lib.det_scores_workspace(F32, 4, (1 << 18) + 1, 0) == 0
     assert lib.det_scores_workspace(3, 4, 1000, 0) == 0
+
+
+@pytest.mark.parametrize("call,k", [(scores_step, 1), (loss_step, 8)])
+def test_step_workspace(lib, call, k):
+    need = lib.det_step_workspace(4, k)
+    assert need > 0
+    assert call(lib, size=need) == NO_DEVICE
+    assert call(lib, size=need - 1) == INVALID
+    assert call(lib, ws=None) == INVALID
+    assert call(lib, ws=P + 8) == INVALID
+    assert lib.det_step_workspace(4, 129) == 0
 
 
 @pytest.mark.parametrize("call", LISTS)
