@@ -114,7 +114,7 @@ def lib():
             "det_scores_workspace": (SZ, [I, U32, U32, U32]),
             "det_token_scores_device": (I, [P, I, U32, U32, U64, P, I, U32, P, P, P, P, P, P, P, SZ, P]),
             "det_token_scores_grad_device": (I, [P, I, U32, U32, U64, P, I, P, P, P, P, U64, P]),
-            "det_step_workspace": (SZ, [U32, U32]),
+            "det_step_workspace": (SZ, [U32, U32, U32]),
             "det_token_scores_step_device": (I, [P, I, U32, U32, U64, P, I, P, P, P, P, P, P, U64, P, P, SZ, P]),
             "det_distill_loss_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P, SZ, P]),
             "det_distill_grad_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, U64, P]),

@@ -878,30 +878,6 @@ DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int
   __syncthreads();
 }
 
-// ---- clusters ------------------------------------------------------------------------
-DI uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-DI uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
-}
-DI void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-DI void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// *p of block `rank` of the cluster, p an address of one's own shared memory
-DI uint32_t remote(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  return r;
-}
-DI void store_remote(uint32_t at, float4 v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-               : "memory");
-}
-
 // what a row's scores are written to (one thread)
 DI void write_stats(float* stats, int row, const RowStats& r, double log_s) {
   float* st = stats + (size_t)row * 4;
@@ -1264,26 +1240,31 @@ DI void store_segment(T* y, int g, int V, int my, F vec) {
 }
 
 // Three kernels.  The first gathers what the gradient's coefficients and the
-// logits at a row's own tokens are, before `out` may overwrite those.  In the
-// second, clusters take rows in turn; each of a cluster's warps holds one
+// logits at a row's own tokens are, before `out` may overwrite those.  The
+// third writes the rows' scores and adds the part of their own tokens.
+//
+// In the second, clusters draw rows; each of a cluster's warps holds one
 // segment of the row, so the row is read once: its exponentials stay in
-// registers until every block has all segments' sums, and are scaled and
-// stored then, while the next row's segment is on its way.  (The entropy's
-// gradient needs y too: it keeps the logits and takes their exponentials
-// again.)  One cluster barrier per row: the sums have two places, and a warp
-// writes to one of them again only behind the barrier of the row between, at
-// which every warp has read it.  The third writes the rows' scores and adds
-// the part of their own tokens.
+// registers until all segments' sums are there, and are scaled and stored
+// then, while the next row's segment is on its way.  (The entropy's gradient
+// needs y too: it keeps the logits and takes their exponentials again.)  A
+// warp sends its sums to every block of the cluster, where an mbarrier counts
+// their bytes: no barrier that all warps stop at, and no fence, which would
+// also wait for the last row's stores and the next segment's copies.  The sums
+// have two places and two mbarriers; a warp sends the row after next only when
+// it has the next row's sums, which every warp sent after it read the row's.
 struct StepWork {
-  float4* coef;  // per row: of the loss over T, or of logprob; of the entropy; 1 where there is nothing but zeros
-  float* z;      // per row and entry: the logit at its token
+  float4* coef;      // per row: of the loss over T, or of minus logprob; of the entropy; 1 where all is zeros
+  float* z;          // per row and entry: the logit at its token
+  uint32_t* ticket;  // rows drawn
 };
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    step_gather_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, StepWork ws) {
-  pdl_trigger();
+    step_gather_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, StepWork ws,
+                       uint32_t first) {
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), l = threadIdx.x & 31, V = L.vocab;
   if (row >= L.n) return;
+  if (row == 0 && l == 0) *ws.ticket = first;
   const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
   const float nan = __int_as_float(0x7fffffff);
   if (te.k) {
@@ -1314,11 +1295,61 @@ DI RowGrad row_grad(float a_g, float a_h, bool zero, const RowStats& r, float c)
   const float a = a_h == 0.0f ? a_g : fadd(a_g, fmul(a_h, fdiv(r.s1, r.s)));
   return {-r.m, c, fmul(a, inv_s), fmul(fmul(-a_h, kLn2), inv_s), zero || r.empty};
 }
+DI uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+DI uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+DI void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+DI uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// the address of one's own shared memory in block `rank` of the cluster
+DI uint32_t remote(uint32_t p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(rank));
+  return r;
+}
+// 16 bytes to a block of the cluster, counted by its mbarrier (in a launch with
+// clusters: without them the instruction is not there)
+DI void send(uint32_t at, uint32_t bar, float4 v) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at),
+      "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
+      : "memory");
+}
+DI bool bar_done(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// waits for the barrier's phase, a second at most
+DI bool bar_wait(uint32_t bar, uint32_t parity) {
+  if (bar_done(bar, parity)) return true;
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do {
+    if (bar_done(bar, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  } while (t - t0 < 1000000000ull);
+  return false;
+}
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads, 2)
-    step_kernel(Logits L, float temp, StepWork ws, float* stats, T* out, unsigned long long out_ld, float one_) {
+    step_kernel(Logits L, float temp, StepWork ws, float* stats, uint32_t* flags, T* out, unsigned long long out_ld,
+                float one_) {
   using G = Seg<T>;
   __shared__ float4 seg[2][kMaxSegs];
+  __shared__ __align__(8) unsigned long long bars[2];
   extern __shared__ __align__(16) uint8_t dyn[];
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int V = L.vocab, w = threadIdx.x >> 5, l = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -1327,59 +1358,70 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool active = g < nseg;
   void* stage = dyn + w * kStageBytes<T>;
   auto at_row = [&](int r) { return static_cast<const T*>(L.x) + (size_t)r * L.ld; };
-  int row = blockIdx.x / size;
-  if (row < L.n && active) stage_issue<T>(stage, at_row(row), g, V);
+  int row = blockIdx.x / size, next = row + clusters;
+  if (active) stage_issue<T>(stage, at_row(row), g, V);
   pdl_trigger();
   const float c = fdiv(kLog2e, temp);
-  const uint32_t table = kExpTable[l];
-  const uint32_t place = remote(&seg[0][g < kMaxSegs ? g : 0], l < (int)size ? l : 0);
-  if (size > 1) {  // every block runs before anyone writes to it
-    cluster_arrive();
-    cluster_wait();
+  const uint32_t table = kExpTable[l], bar = shared_at(bars);
+  if (threadIdx.x == 0) {
+    // a lone block's warps arrive themselves
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\nmbarrier.init.shared::cta.b64 [%0 + 8], %1;" ::"r"(bar),
+                 "r"(size > 1 ? 1 : nseg)
+                 : "memory");
+    if (size > 1) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  bool gathered = false;
-  float4 coef;
-  for (int turn = 0; row < L.n; row += clusters, turn ^= 1) {
-    uint4 raw[G::NV];
-    float v[ENTROPY ? 1 : kPerLane];
-    if (gathered) coef = ws.coef[row];
-    float m_seg = -INFINITY, s_seg = 0.0f, w_seg = 0.0f;
-    if (active) {
+  // the barriers are set before anyone sends to them
+  if (size > 1) cluster_sync();
+  else __syncthreads();
+  pdl_wait();  // the first kernel's results are there, and its reads done
+  const uint32_t to = l < (int)size ? l : 0;
+  const uint32_t place = remote(shared_at(&seg[0][g < kMaxSegs ? g : 0]), to), to_bar = remote(bar, to);
+  if (active) {
+    for (int turn = 0; row < L.n; turn++) {
+      const int half = turn & 1;
+      uint4 raw[G::NV];
+      float v[ENTROPY ? 1 : kPerLane];
+      // block 0's first warp draws the row after next, which goes with its sums
+      uint32_t after = 0;
+      if (g == 0 && l == 0) after = atomicAdd(ws.ticket, 1u);
+      if (size > 1 && threadIdx.x == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar + 8 * half), "r"(16 * nseg)
+                     : "memory");
+      const float4 coef = ws.coef[row];
       stage_take<T>(stage, misaligned(at_row(row)), raw);
-      if (row + clusters < L.n) stage_issue<T>(stage, at_row(row + clusters), g, V);
+      if (next < L.n) stage_issue<T>(stage, at_row(next), g, V);
       Range<T> range;
 #pragma unroll
       for (int i = 0; i < G::NV; i++) range.take(raw[i]);
-      m_seg = redux_max(range.high());
-      s_seg = segment_sums<T, !ENTROPY>(raw, V - g * kSeg, m_seg, redux_min(range.low()), c, table, one_, v);
-      w_seg = __shfl_sync(kFull, s_seg, 16);
-      s_seg = __shfl_sync(kFull, s_seg, 0);
-      if (l < (int)size)
-        store_remote(place + turn * (uint32_t)sizeof(seg[0]), make_float4(m_seg, s_seg, w_seg, 0.0f));
-    }
-    if (size > 1) {
-      cluster_arrive();
-      cluster_wait();
-    } else {
-      __syncthreads();
-    }
-    if (!gathered) {  // the first kernel's results, and its reads are done
-      pdl_wait();
-      gathered = true;
-      coef = ws.coef[row];
-    }
-    const RowStats r = finish_row(join_segments(
-        [&](int i) {
-          const float4 f = seg[turn][i];
-          return Sums{f.x, f.y, f.z};
-        },
-        nseg, c, table, one_));
-    const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
-    if (rank == 0 && threadIdx.x == 0) {
-      float* st = stats + (size_t)row * 4;
-      st[0] = r.m, st[1] = r.s, st[2] = r.s1;
-    }
-    if (active) {
+      const float m_seg = redux_max(range.high());
+      const float sum = segment_sums<T, !ENTROPY>(raw, V - g * kSeg, m_seg, redux_min(range.low()), c, table, one_, v);
+      const float s_seg = __shfl_sync(kFull, sum, 0), w_seg = __shfl_sync(kFull, sum, 16);
+      after = __shfl_sync(kFull, after, 0);
+      const float4 mine = make_float4(m_seg, s_seg, w_seg, __uint_as_float(after));
+      if (size > 1) {
+        if (l < (int)size) send(place + half * (uint32_t)sizeof(seg[0]), to_bar + 8 * half, mine);
+      } else if (l == 0) {
+        seg[half][g] = mine;
+        asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar + 8 * half) : "memory");
+      }
+      // The wait ends: the other warps run, and send what this one waits for
+      // without waiting for this row.  Should it not, the row is given up as
+      // NaN and the warp stops after the next.
+      const bool there = __all_sync(kFull, bar_wait(bar + 8 * half, (turn >> 1) & 1));
+      if (!there && l == 0 && flags) atomicOr(flags, (uint32_t)DET_SCORE_TIMEOUT);
+      RowStats r = finish_row(join_segments(
+          [&](int i) {
+            const float4 f = seg[half][i];
+            return Sums{f.x, f.y, f.z};
+          },
+          nseg, c, table, one_));
+      const int drawn = (int)__float_as_uint(seg[half][0].w);
+      if (!there) r.m = r.s = r.s1 = __int_as_float(0x7fffffff), r.empty = false;
+      const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
+      if (g == 0 && l == 0) {
+        float* st = stats + (size_t)row * 4;
+        st[0] = r.m, st[1] = r.s, st[2] = r.s1;
+      }
       const f2 one = pk(one_, one_), cc = pk(c, c);
       const float y_seg = segment_y(m_seg, r.m, c);
       const float f = fmul(un(exp2_warp<true>(pk(y_seg, y_seg), table, one).e).x, rg.as);
@@ -1407,11 +1449,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       };
       T* y = out + (size_t)row * out_ld;
       store_segment<T>(y, g, V, misaligned(y), vec);
+      row = next;
+      next = there ? drawn : L.n;
     }
   }
-  if (size > 1) {  // nobody leaves while another block may still write to it
-    cluster_arrive();
-    cluster_wait();
+  // nobody leaves while another block may still send to it
+  if (size > 1) {
+    __syncwarp();
+    cluster_sync();
   }
 }
 template <typename T, bool ENTROPY>
@@ -1473,9 +1518,26 @@ cudaError_t by_dtype(int dtype, F f) {
   }
 }
 
-// Clusters of `c` blocks that the current device holds at once, at least 1
-// (cached: the answer depends on the kernel and the launch alone).
+// Blocks of a kernel that the current device holds at once (cached: the answer
+// depends on the kernel and the launch alone).
+int resident_blocks(const void* kern, int threads, size_t smem) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int, size_t>, int> known;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[{kern, dev, threads, smem}];
+  if (n > 0) return n;
+  int per = 0, sms = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, smem) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    cudaGetLastError();
+  return n = per * sms > 0 ? per * sms : 1;
+}
+
+// Clusters of c blocks that the current device holds at once, likewise.
 int resident_clusters(const void* kern, int c, int threads, size_t smem) {
+  if (c == 1) return resident_blocks(kern, threads, smem);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 1;
   static std::mutex mu;
@@ -1494,11 +1556,8 @@ int resident_clusters(const void* kern, int c, int threads, size_t smem) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int got = 0;
-  if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess || got < 1) {
-    cudaGetLastError();
-    got = 1;
-  }
-  return n = got;
+  if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess) cudaGetLastError();
+  return n = got > 0 ? got : 1;
 }
 // launches `clusters` clusters of c blocks, with programmatic stream
 // serialization
@@ -1552,7 +1611,7 @@ cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int 
   const size_t smem = kSegWarps * kStageBytes<T>;
   if (cudaError_t e = raise_smem_cap((const void*)segments, smem)) return e;
   const long long nseg = (L.vocab + kSeg - 1) / kSeg, blocks = (L.n * nseg + kSegWarps - 1) / kSegWarps;
-  const int fit = resident_clusters((const void*)segments, 1, kSegThreads, smem);
+  const int fit = resident_blocks((const void*)segments, kSegThreads, smem);
   Workspace ws;
   ws.seg = static_cast<float4*>(workspace);
   ws.gmax = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256(L.n * nseg * sizeof(float4)));
@@ -1598,13 +1657,24 @@ cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* 
   });
 }
 
-size_t step_workspace_bytes(size_t n, int k) { return align256(n * sizeof(float4)) + align256(n * k * sizeof(float)); }
+size_t step_workspace_bytes(size_t n, int k) {
+  return align256(n * sizeof(float4)) + align256(n * k * sizeof(float)) + align256(sizeof(uint32_t));
+}
 template <typename T, bool ENTROPY>
 cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
                     const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
                     unsigned long long out_ld) {
-  const StepWork ws{static_cast<float4*>(workspace),
-                    reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256(L.n * sizeof(float4)))};
+  const size_t n = L.n, k = te.k ? te.k : 1;
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  auto take = [&](size_t bytes) {
+    uint8_t* p = at;
+    at += align256(bytes);
+    return p;
+  };
+  StepWork ws;
+  ws.coef = reinterpret_cast<float4*>(take(n * sizeof(float4)));
+  ws.z = reinterpret_cast<float*>(take(n * k * sizeof(float)));
+  ws.ticket = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t)));
   const auto kern = step_kernel<T, ENTROPY>;
   // a warp per segment
   const int nseg = (L.vocab + kSeg - 1) / kSeg, c = (nseg + kWarps - 1) / kWarps, warps = (nseg + c - 1) / c;
@@ -1612,12 +1682,13 @@ cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
   if (cudaError_t e = raise_smem_cap((const void*)kern, smem)) return e;
   if (c > 8)
     if (cudaError_t e = allow_large_clusters((const void*)kern)) return e;
-  const int fit = resident_clusters((const void*)kern, c, 32 * warps, smem);
-  step_gather_kernel<T><<<(L.n + kWarps - 1) / kWarps, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, ws);
+  const int fit = resident_clusters((const void*)kern, c, 32 * warps, smem), clusters = L.n < fit ? L.n : fit;
+  step_gather_kernel<T>
+      <<<(L.n + kWarps - 1) / kWarps, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, ws, 2 * clusters);
   if (cudaError_t e = cudaGetLastError()) return e;
   T* y = static_cast<T*>(out);
-  if (cudaError_t e = launch_clusters(s, kern, L.n < fit ? L.n : fit, c, 32 * warps, smem, L, temp, ws, o.stats, y,
-                                      out_ld, 1.0f))
+  if (cudaError_t e = launch_clusters(s, kern, clusters, c, 32 * warps, smem, L, temp, ws, o.stats, o.flags, y, out_ld,
+                                      1.0f))
     return e;
   const Launch launch{s, nullptr, nullptr, true};
   return launch_k(launch, step_rows_kernel<T, ENTROPY>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes, te, temp,
@@ -1721,8 +1792,9 @@ size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top)
   return workspace_bytes(dtype, (int)n, (int)vocab, (int)top);
 }
 
-size_t det_step_workspace(uint32_t n, uint32_t k) {
-  return n > DET_SCORE_MAX_ROWS || k > DET_MAX_TOP ? 0 : step_workspace_bytes(n, k ? (int)k : 1);
+size_t det_step_workspace(uint32_t n, uint32_t vocab, uint32_t k) {
+  if (n > DET_SCORE_MAX_ROWS || vocab > kMaxVocab || k > DET_MAX_TOP) return 0;
+  return step_workspace_bytes(n, k ? (int)k : 1);
 }
 
 det_status det_token_scores_device(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld,

@@ -156,7 +156,7 @@ def token_scores_step(logits, tokens, grad_logprob=None, grad_entropy=None, out=
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     logprob, entropy, stats = _new(logits, n), _new(logits, n), _new(logits, n, 4)
-    work, size = _workspace(logits, lib().det_step_workspace(n, 1))
+    work, size = _workspace(logits, lib().det_step_workspace(n, vocab, 1))
     _call("det_token_scores_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
           _IDS[tokens.dtype], gl, ge, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld,
           None, work.data_ptr(), size)
@@ -200,7 +200,7 @@ def distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperature: fl
     g = _vector(grad_loss, logits, "grad_loss", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     loss, stats = _new(logits, n), _new(logits, n, 4)
-    work, size = _workspace(logits, lib().det_step_workspace(n, lists[4]))
+    work, size = _workspace(logits, lib().det_step_workspace(n, vocab, lists[4]))
     _call("det_distill_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
           temperature, g, loss.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld, None, work.data_ptr(), size)
     return DistillLoss(loss, stats), out

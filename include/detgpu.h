@@ -347,7 +347,7 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  * themselves (same pointer and stride), or side by side with them in rows of
  * one stride; any other overlap is DET_ERR_INVALID_ARGUMENT. */
 enum { DET_DTYPE_F32 = 0, DET_DTYPE_F16 = 1, DET_DTYPE_BF16 = 2 };
-enum { DET_SCORE_NONFINITE = 2, DET_SCORE_BAD_TOKEN = 64 };
+enum { DET_SCORE_NONFINITE = 2, DET_SCORE_TIMEOUT = 32, DET_SCORE_BAD_TOKEN = 64 };
 #define DET_MAX_TOP 128u
 #define DET_SCORE_MAX_ROWS (1u << 26)
 #define DET_MIN_TEMPERATURE 1e-6f
@@ -366,7 +366,7 @@ det_status det_distill_loss(det_session* s, const uint32_t* rows, uint32_t n, co
  * list, 1 for scores); 16-byte aligned.  Calls that may overlap need one each;
  * what it holds between calls does not matter. */
 size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top);
-size_t det_step_workspace(uint32_t n, uint32_t k);
+size_t det_step_workspace(uint32_t n, uint32_t vocab, uint32_t k);
 /* log probability of tokens[i], entropy, and the `top` (<= DET_MAX_TOP, <=
  * vocab) most likely tokens of row i with their log probabilities, most
  * likely first, equal ones in the order of their ids: n x top each */

@@ -113,13 +113,13 @@ def test_workspace(lib, call):
 
 @pytest.mark.parametrize("call,k", [(scores_step, 1), (loss_step, 8)])
 def test_step_workspace(lib, call, k):
-    need = lib.det_step_workspace(4, k)
+    need = lib.det_step_workspace(4, 1000, k)
     assert need > 0
     assert call(lib, size=need) == NO_DEVICE
     assert call(lib, size=need - 1) == INVALID
     assert call(lib, ws=None) == INVALID
     assert call(lib, ws=P + 8) == INVALID
-    assert lib.det_step_workspace(4, 129) == 0
+    assert lib.det_step_workspace(4, 1000, 129) == 0
 
 
 @pytest.mark.parametrize("call", LISTS)
