@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -475,8 +476,9 @@ DI float segment_y(float ms, float m, float c) {
   return ms == -INFINITY ? kYLow : fmaxf(fmul(fsub(ms, m), c), kYLow);
 }
 // joins a row's segments (one warp; the result in every lane): at(i) gives
-// segment i's sums
-template <typename F>
+// segment i's sums.  WHOLE: w too; otherwise w only says if the row is bad (0
+// or NaN).
+template <bool WHOLE, typename F>
 DI Sums join_segments(F at, int nseg, float c, uint32_t table, float one) {
   const int l = threadIdx.x & 31;
   Sums t[kMaxSegs / 32];
@@ -495,9 +497,14 @@ DI Sums join_segments(F at, int nseg, float c, uint32_t table, float one) {
     const float f = un(exp2_warp<true>(pk(y, y), table, pk(one, one)).e).x;
     s = fadd(s, fmul(f, t[i].s));
     // sum of 2^(y_j + y) (y_j + y) = f (w + y s); NaN stays NaN
-    w = fadd(w, fmul(f, fadd(t[i].w, fmul(y, t[i].s))));
+    if constexpr (WHOLE) w = fadd(w, fmul(f, fadd(t[i].w, fmul(y, t[i].s))));
+    else if (__any_sync(kFull, !(t[i].w == t[i].w))) w = __int_as_float(0x7fffffff);
   }
-  return {m, warp_sum(s), warp_sum(w)};
+  if constexpr (WHOLE) {
+    const float v = warp_sum2(s, w);
+    return {m, __shfl_sync(kFull, v, 0), __shfl_sync(kFull, v, 16)};
+  }
+  return {m, warp_sum(s), w};
 }
 
 struct RowStats {
@@ -988,7 +995,7 @@ __global__ void __launch_bounds__(kRowThreads, 7)
   double log_s;
   auto scores = [&]() {
     const float4* seg = ws.seg + (size_t)row * nseg;
-    r = finish_row(join_segments(
+    r = finish_row(join_segments<true>(
         [&](int i) {
           const float4 f = seg[i];
           return Sums{f.x, f.y, f.z};
@@ -1218,6 +1225,12 @@ DI void store_segment(T* y, int g, int V, int my, F vec) {
         if (at + j >= lo && at + j < hi) y[at + j] = from_f32<T>(f[j]);
     }
   };
+  if (my == 0 && lo + kSeg <= V) {
+    uint4* p = reinterpret_cast<uint4*>(y + lo) + l;
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) p[32 * i] = vec(i);
+    return;
+  }
   if (my == 0) {
 #pragma unroll
     for (int i = 0; i < G::NV; i++) put(lo + (32 * i + l) * VEC, vec(i));
@@ -1409,12 +1422,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       // NaN and the warp stops after the next.
       const bool there = __all_sync(kFull, bar_wait(bar + 8 * half, (turn >> 1) & 1));
       if (!there && l == 0 && flags) atomicOr(flags, (uint32_t)DET_SCORE_TIMEOUT);
-      RowStats r = finish_row(join_segments(
-          [&](int i) {
-            const float4 f = seg[half][i];
-            return Sums{f.x, f.y, f.z};
-          },
-          nseg, c, table, one_));
+      auto sums_of = [&](int i) {
+        const float4 f = seg[half][i];
+        return Sums{f.x, f.y, f.z};
+      };
+      // the sum of 2^y y is for the entropy's gradient, and for one warp to write
+      RowStats r = finish_row(ENTROPY || g == 0 ? join_segments<true>(sums_of, nseg, c, table, one_)
+                                                : join_segments<false>(sums_of, nseg, c, table, one_));
       const int drawn = (int)__float_as_uint(seg[half][0].w);
       if (!there) r.m = r.s = r.s1 = __int_as_float(0x7fffffff), r.empty = false;
       const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
@@ -1748,8 +1762,12 @@ det_status check_workspace(const void* workspace, size_t size, size_t need) {
   return workspace && (uintptr_t)workspace % 16 == 0 && size >= need ? DET_OK : DET_ERR_INVALID_ARGUMENT;
 }
 det_status check_device() {
+  static std::atomic<bool> seen{false};
+  if (seen.load(std::memory_order_relaxed)) return DET_OK;
   int cnt = 0;
-  return cudaGetDeviceCount(&cnt) != cudaSuccess || cnt == 0 ? DET_ERR_NO_DEVICE : DET_OK;
+  if (cudaGetDeviceCount(&cnt) != cudaSuccess || cnt == 0) return DET_ERR_NO_DEVICE;
+  seen.store(true, std::memory_order_relaxed);
+  return DET_OK;
 }
 det_status launched(cudaError_t e) {
   return e == cudaSuccess ? DET_OK : e == cudaErrorMemoryAllocation ? DET_ERR_DEVICE_OOM : DET_ERR_CUDA;

@@ -19,7 +19,6 @@ There is no CPU fallback.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple, Optional
 
 import torch
@@ -29,8 +28,12 @@ from . import DetError, lib
 __all__ = ["TokenScores", "DistillLoss", "token_scores", "token_scores_grad", "token_scores_step", "distill_loss",
            "distill_grad", "distill_step"]
 
+_F32 = torch.float32
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _IDS = {torch.int32: 4, torch.int64: 8}
+# the handle of a device's current stream (0.1 us, where a Stream object takes 2)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class TokenScores(NamedTuple):
@@ -62,21 +65,20 @@ def _logits(x, what="logits"):
 
 def _on(t, logits, what, shape, dtypes, rows=False):
     """The data pointer of `t`, checked; rows: only its rows need be dense."""
-    if t.device != logits.device or tuple(t.shape) != shape or t.dtype not in dtypes:
+    if t.shape != shape or t.dtype not in dtypes or t.device != logits.device:
         raise ValueError(f"{what} must be {list(shape)} of {' or '.join(str(d)[6:] for d in dtypes)} on {logits.device}")
-    if not (t.stride(-1) == 1 or t.shape[-1] == 1 if rows else t.is_contiguous()):
+    if not (t.stride(-1) == 1 or t.shape[-1] <= 1 if rows else t.is_contiguous()):
         raise ValueError(f"{what} must be {'dense in each row' if rows else 'contiguous'}")
     return t.data_ptr()
 
 
 def _vector(t, logits, what, n):
-    return None if t is None else _on(t, logits, what, (n,), (torch.float32,))
+    return None if t is None else _on(t, logits, what, (n,), (_F32,))
 
 
 def _grad_out(logits, out, n, vocab):
     if out is None:
-        out = torch.empty((n, vocab), dtype=logits.dtype, device=logits.device)
-        return out, vocab
+        return logits.new_empty((n, vocab)), vocab
     _on(out, logits, "out", (n, vocab), (logits.dtype,), rows=True)
     return out, out.stride(0) if n > 1 else vocab
 
@@ -85,8 +87,8 @@ def _lists(ids, teacher, logits, n):
     if ids.dim() != 2 or teacher.dim() != 2:
         raise ValueError("teacher_ids and teacher_logits must be [rows, entries]")
     k = ids.shape[1]
-    pi = _on(ids, logits, "teacher_ids", (n, k), tuple(_IDS), rows=True)
-    pt = _on(teacher, logits, "teacher_logits", (n, k), tuple(_DTYPES), rows=True)
+    pi = _on(ids, logits, "teacher_ids", (n, k), _IDS, rows=True)
+    pt = _on(teacher, logits, "teacher_logits", (n, k), _DTYPES, rows=True)
     li, lt = (t.stride(0) if n > 1 else k for t in (ids, teacher))
     if li != lt:
         raise ValueError("teacher_ids and teacher_logits must have the same distance between rows")
@@ -95,20 +97,23 @@ def _lists(ids, teacher, logits, n):
 
 def _call(name, logits, *args):
     # the library works on the calling thread's current device
-    dev = logits.device
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    with contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
-        st = getattr(lib(), name)(*args, stream)
+    index = logits.device.index
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == index:
+        st = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, _stream(index))
     if st:
         raise DetError(st, name)
 
 
 def _new(logits, *shape):
-    return torch.empty(shape, dtype=torch.float32, device=logits.device)
+    return logits.new_empty(shape, dtype=_F32)
 
 
 def _workspace(logits, size):
-    return torch.empty(size, dtype=torch.uint8, device=logits.device), size
+    return logits.new_empty(size, dtype=torch.uint8), size
 
 
 def token_scores(logits, tokens, top: int = 0) -> TokenScores:
@@ -116,13 +121,13 @@ def token_scores(logits, tokens, top: int = 0) -> TokenScores:
     ``top`` (at most 128) most likely tokens, most likely first and equal ones
     in the order of their ids."""
     n, vocab, ld = _logits(logits)
-    tok = _on(tokens, logits, "tokens", (n,), tuple(_IDS))
+    tok = _on(tokens, logits, "tokens", (n,), _IDS)
     logprob, entropy, stats = _new(logits, n), _new(logits, n), _new(logits, n, 4)
     ids = lps = None
     if top:
         if top < 0:
             raise ValueError("top must not be negative")
-        ids = torch.empty((n, top), dtype=torch.int32, device=logits.device)
+        ids = logits.new_empty((n, top), dtype=torch.int32)
         lps = _new(logits, n, top)
     work, size = _workspace(logits, lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, top))
     _call("det_token_scores_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
@@ -136,8 +141,8 @@ def token_scores_grad(logits, tokens, stats, grad_logprob=None, grad_entropy=Non
     the ``stats`` that :func:`token_scores` gave for the same logits.  ``out``
     may be the logits themselves."""
     n, vocab, ld = _logits(logits)
-    tok = _on(tokens, logits, "tokens", (n,), tuple(_IDS))
-    ps = _on(stats, logits, "stats", (n, 4), (torch.float32,))
+    tok = _on(tokens, logits, "tokens", (n,), _IDS)
+    ps = _on(stats, logits, "stats", (n, 4), (_F32,))
     gl = _vector(grad_logprob, logits, "grad_logprob", n)
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
@@ -151,7 +156,7 @@ def token_scores_step(logits, tokens, grad_logprob=None, grad_entropy=None, out=
     that reads the logits once: ``(TokenScores, gradient)``.  With
     ``grad_logprob`` = -1/n it is the step of the mean code length."""
     n, vocab, ld = _logits(logits)
-    tok = _on(tokens, logits, "tokens", (n,), tuple(_IDS))
+    tok = _on(tokens, logits, "tokens", (n,), _IDS)
     gl = _vector(grad_logprob, logits, "grad_logprob", n)
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
@@ -184,7 +189,7 @@ def distill_grad(logits, teacher_ids, teacher_logits, stats, grad_loss, temperat
     be the logits themselves."""
     n, vocab, ld = _logits(logits)
     lists = _lists(teacher_ids, teacher_logits, logits, n)
-    ps = _on(stats, logits, "stats", (n, 4), (torch.float32,))
+    ps = _on(stats, logits, "stats", (n, 4), (_F32,))
     g = _vector(grad_loss, logits, "grad_loss", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     _call("det_distill_grad_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
