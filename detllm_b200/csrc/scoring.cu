@@ -1649,10 +1649,17 @@ cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
                     const GradIn& in, void* out, unsigned long long out_ld) {
   constexpr int VEC = Seg<T>::VEC;
   const int nvec = (L.vocab + VEC - 1) / VEC + 1;  // one more where a row starts inside a vector
-  // up to 8 runs per warp, fewer where that would leave SMs without a block
-  const int step = kThreads * kGradUnroll;
-  int per = 8 * step;
-  while (per > step && (long long)L.n * ((nvec + per - 1) / per) < 8 * device_sms()) per -= step;
+  // Runs per warp, up to 8: the waves of blocks, times a block's runs and what
+  // it costs beside them (half a run's time; a list takes about two)
+  const int step = kThreads * kGradUnroll, fit = resident_blocks((const void*)grad_kernel<T, ENTROPY>, kThreads, 0);
+  int per = step;
+  float least = 0.0f;
+  for (int runs = 1; runs <= 8; runs++) {
+    const long long all = (long long)L.n * ((nvec + runs * step - 1) / (runs * step));
+    const float cost = (float)((all + fit - 1) / fit) * (runs + (te.k ? 2.0f : 0.5f));
+    if (runs == 1 || cost < least) least = cost, per = runs * step;
+  }
+  // and less than a run of each warp where SMs would be without a block
   while (per > kGradRun && (long long)L.n * ((nvec + per - 1) / per) < device_sms()) per /= 2;
   const int blocks = (nvec + per - 1) / per;
   for (int r = 0; r < L.n; r += 65535) {
