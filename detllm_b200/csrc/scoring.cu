@@ -1726,13 +1726,15 @@ cudaError_t launch_step(cudaStream_t s, int dtype, const Logits& L, const void* 
 }
 
 // ---- argument checks ----------------------------------------------------------------
+constexpr uint64_t kMaxLd = 1ull << 36;  // with DET_SCORE_MAX_ROWS rows of 4 bytes: below 2^64
+
 size_t dtype_size(int dtype) { return dtype == DET_DTYPE_F32 ? 4 : 2; }
 
 det_status check_logits(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld) {
   if (!logits || dtype < DET_DTYPE_F32 || dtype > DET_DTYPE_BF16) return DET_ERR_INVALID_ARGUMENT;
   if (vocab == 0) return DET_ERR_CDF_EMPTY;
   if (vocab > kMaxVocab) return DET_ERR_CDF_TOO_MANY_SYMBOLS;
-  if (n > DET_SCORE_MAX_ROWS || ld > (1ull << 40)) return DET_ERR_INVALID_ARGUMENT;
+  if (n > DET_SCORE_MAX_ROWS || ld > kMaxLd) return DET_ERR_INVALID_ARGUMENT;
   if ((uintptr_t)logits % dtype_size(dtype)) return DET_ERR_INVALID_ARGUMENT;
   return DET_OK;
 }
@@ -1740,13 +1742,13 @@ det_status check_logits(const void* logits, int dtype, uint32_t n, uint32_t voca
 // strides side by side, or ranges that do not meet
 det_status check_grad(const void* logits, int dtype, uint32_t n, uint32_t vocab, uint64_t ld, const void* grad,
                       uint64_t grad_ld) {
-  if (!grad || (n > 1 && grad_ld < vocab) || grad_ld > (1ull << 40)) return DET_ERR_INVALID_ARGUMENT;
+  if (!grad || (n > 1 && grad_ld < vocab) || grad_ld > kMaxLd) return DET_ERR_INVALID_ARGUMENT;
   const size_t sz = dtype_size(dtype);
   if ((uintptr_t)grad % sz) return DET_ERR_INVALID_ARGUMENT;
   const uintptr_t a = (uintptr_t)logits, b = (uintptr_t)grad;
   if (a == b) return n == 1 || ld == grad_ld ? DET_OK : DET_ERR_INVALID_ARGUMENT;
   const size_t an = ((size_t)(n - 1) * ld + vocab) * sz, bn = ((size_t)(n - 1) * grad_ld + vocab) * sz;
-  if (a + an <= b || b + bn <= a) return DET_OK;
+  if (b > a ? b - a >= an : a - b >= bn) return DET_OK;
   if (n == 1 || ld != grad_ld) return DET_ERR_INVALID_ARGUMENT;
   const size_t pitch = ld * sz, off = (b > a ? b - a : pitch - (a - b) % pitch) % pitch, row = vocab * sz;
   return off >= row && off + row <= pitch ? DET_OK : DET_ERR_INVALID_ARGUMENT;
@@ -1761,7 +1763,7 @@ det_status check_list(const void* ids, int id_bytes, const void* teacher, int te
   if (!teacher || teacher_dtype < DET_DTYPE_F32 || teacher_dtype > DET_DTYPE_BF16 ||
       (uintptr_t)teacher % dtype_size(teacher_dtype))
     return DET_ERR_INVALID_ARGUMENT;
-  if (k == 0 || k > DET_MAX_TOP || (n > 1 && ld < k) || ld > (1ull << 40)) return DET_ERR_INVALID_ARGUMENT;
+  if (k == 0 || k > DET_MAX_TOP || (n > 1 && ld < k) || ld > kMaxLd) return DET_ERR_INVALID_ARGUMENT;
   if (!(temperature >= DET_MIN_TEMPERATURE && temperature <= DET_MAX_TEMPERATURE)) return DET_ERR_INVALID_ARGUMENT;
   return DET_OK;
 }

@@ -323,6 +323,8 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  *   list entry: id < 0, u -inf not a valid entry; u NaN or +inf: as a bad id
  *   no valid entry in a list   loss 0 and gradient 0, whatever the logits
  *   an id listed twice         two terms of the loss; its gradient has both
+ *   (a bounded wait of a step call's kernel ran out: DET_SCORE_TIMEOUT and NaN;
+ *   it is not expected to)
  * A probability below 2^-123 of the row's largest counts as 0.
  *
  * Results are deterministic, and a row's are the same bits in whatever batch

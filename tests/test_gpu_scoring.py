@@ -594,6 +594,110 @@ def test_backward_of_a_user_s_own_function(env):
     assert float((own - leaf.grad).abs().max()) < 1e-6
 
 
+def test_lists_of_wider_rows_and_of_one_row(env):
+    """Lists that are columns of a wider tensor; one list for every row is
+    refused (its rows do not lie apart) until it is laid out."""
+    D, torch, sc = env
+    x, _, g = make(torch, 6, 700, torch.bfloat16, 4)
+    ids = torch.randint(0, 700, (6, 40), generator=g, device="cuda")
+    u = torch.randn(6, 40, generator=g, device="cuda")
+    got = sc.distill_loss(x, ids[:, 3:20], u[:, 3:20], 2.0)
+    want = sc.distill_loss(x, ids[:, 3:20].contiguous(), u[:, 3:20].contiguous(), 2.0)
+    assert torch.equal(got.loss, want.loss)
+    with pytest.raises(D.DetError):
+        sc.distill_loss(x, ids[:1].expand(6, 40), u[:1].expand(6, 40))
+    with pytest.raises(ValueError):
+        sc.distill_loss(x, ids[:, 3:20], u[:, 3:20].contiguous())
+    with pytest.raises(ValueError):
+        sc.distill_loss(x.t(), ids, u)
+    with pytest.raises(D.DetError):
+        sc.token_scores(x, torch.zeros(6, dtype=torch.int64, device="cuda"), top=129)
+
+
+@pytest.mark.parametrize("t", [1e-6, 1e-3, 1e3, 1e6])
+def test_extreme_temperatures(env, t):
+    _, torch, sc = env
+    x, _, g = make(torch, 5, 5000, torch.float32, 9)
+    ids, u = lists(torch, x, 33, g, torch.float32, "full")
+    gr = torch.randn(5, generator=g, device="cuda")
+    t32 = float(np.float32(t))  # the library takes an f32
+    _, _, _, _, loss, tol = distill_ref(torch, x.double(), ids, u, t32)
+    step, grad = sc.distill_step(x, ids, u, gr, t)
+    close(torch, step.loss, loss, tol, "loss")
+    ref, tolg = distill_grad_ref(torch, x.double(), ids, u, t32, gr, x.dtype)
+    close(torch, grad, ref, tolg, "step")
+    close(torch, sc.distill_grad(x, ids, u, step.stats, gr, t), ref, tolg, "grad")
+
+
+def test_one_token_in_every_entry_of_a_list(env):
+    _, torch, sc = env
+    x, _, g = make(torch, 3, 40000, torch.float16, 10)
+    ids = torch.full((3, 128), 39999, device="cuda")
+    u = torch.randn(3, 128, generator=g, device="cuda")
+    gr = torch.ones(3, device="cuda")
+    step, grad = sc.distill_step(x, ids, u, gr)
+    _, _, _, _, loss, tol = distill_ref(torch, x.double(), ids, u, 1.0)
+    close(torch, step.loss, loss, tol, "loss")
+    ref, tolg = distill_grad_ref(torch, x.double(), ids, u, 1.0, gr, x.dtype)
+    close(torch, grad, ref, tolg, "grad")
+
+
+FIRST = """
+import torch
+from detllm_b200 import scoring as sc
+x = torch.randn(9, 40001, device="cuda"); t = torch.randint(0, 40001, (9,), device="cuda")
+g = torch.ones(9, device="cuda"); graph = torch.cuda.CUDAGraph(); torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    f = sc.token_scores(x, t, top=20)
+    s, d = sc.token_scores_step(x, t, g)
+    l, e = sc.distill_step(x, f.top_ids, f.top_logprobs, g, 2.0)
+    h = sc.token_scores_grad(x, t, f.stats, g, g)
+graph.replay(); torch.cuda.synchronize()
+f2 = sc.token_scores(x, t, top=20)
+assert all(torch.equal(a, b) for a, b in zip(f, f2))
+assert torch.equal(d, sc.token_scores_step(x, t, g)[1])
+assert torch.equal(e, sc.distill_step(x, f2.top_ids, f2.top_logprobs, g, 2.0)[1])
+assert torch.equal(h, sc.token_scores_grad(x, t, f2.stats, g, g))
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(env):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+def test_host_threads_at_once(env):
+    """Calls from several host threads, each on its own stream."""
+    import threading
+
+    _, torch, sc = env
+    sets = [make(torch, 40, 30011, torch.bfloat16, 20 + i) for i in range(4)]
+    one = torch.ones(40, device="cuda")
+    want = [(sc.token_scores(x, t, top=9), sc.token_scores_step(x, t, one, one)[1]) for x, t, _ in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        x, t, _ = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                f, d = sc.token_scores(x, t, top=9), sc.token_scores_step(x, t, one, one)[1]
+            torch.cuda.current_stream().synchronize()
+        if not (all(torch.equal(a, b) for a, b in zip(f, want[i][0])) and torch.equal(d, want[i][1])):
+            bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+
+
 # ---- sessions, and a run of all of them together ---------------------------------------------
 
 
