@@ -25,7 +25,6 @@
 #include <cstring>
 #include <map>
 #include <mutex>
-#include <set>
 #include <tuple>
 #include <type_traits>
 
@@ -1549,29 +1548,64 @@ int resident_blocks(const void* kern, int threads, size_t smem) {
   return n = per * sms > 0 ? per * sms : 1;
 }
 
-// Clusters of c blocks that the current device holds at once, likewise.
-int resident_clusters(const void* kern, int c, int threads, size_t smem) {
-  if (c == 1) return resident_blocks(kern, threads, smem);
+// How a kernel with a warp per segment takes rows of nseg segments: clusters of
+// c blocks of `warps` warps, `fit` of which the current device holds at once.
+// Of 4 to 8 warps per block (as many as segments, if those are fewer; 16 blocks
+// per cluster at most) the fewest that hold 93% of the most rows at once: a
+// row's segments wait for one another, so an SM is kept busy by blocks of
+// several rows.  4,096 rows of 128,256 bf16 logits: 570 us in 31 clusters of 16
+// blocks of 4 warps, 609 in 33 of 8 of 8; but of 151,936: 761 us in 26 of 10 of
+// 8, 947 in 24 of 15 of 5.  Below 4 warps more of the time goes into the sends:
+// 1,024 rows of 65,000 take 126 us in blocks of 2, 85 in blocks of 4.  Cached,
+// likewise.
+struct ClusterPlan {
+  int c = 0, warps = 0, fit = 0;
+};
+cudaError_t cluster_plan(const void* kern, int nseg, size_t stage, ClusterPlan* out) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (cudaError_t e = raise_smem_cap(kern, kWarps * stage)) return e;
   static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int, int, size_t>, int> known;
+  static std::map<std::tuple<const void*, int, int>, ClusterPlan> known;
   std::lock_guard<std::mutex> lock(mu);
-  int& n = known[{kern, dev, c, threads, smem}];
-  if (n > 0) return n;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)c);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int got = 0;
-  if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess) cudaGetLastError();
-  return n = got > 0 ? got : 1;
+  ClusterPlan& best = known[{kern, dev, nseg}];
+  if (best.fit == 0) {
+    // clusters above 8 blocks have to be allowed
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
+    ClusterPlan plans[kWarps];
+    int n = 0, most = 0;
+    for (int w = nseg < 4 ? nseg : 4; w <= kWarps; w++) {
+      ClusterPlan p;
+      p.c = (nseg + w - 1) / w;
+      p.warps = (nseg + p.c - 1) / p.c;
+      if (p.c > 16 || p.warps != w) continue;
+      if (p.c == 1) {
+        p.fit = resident_blocks(kern, 32 * w, w * stage);
+      } else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)p.c);
+        cfg.blockDim = dim3((unsigned)(32 * w));
+        cfg.dynamicSmemBytes = w * stage;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.c;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&p.fit, kern, &cfg) != cudaSuccess) {
+          cudaGetLastError();
+          continue;
+        }
+      }
+      plans[n++] = p;
+      most = most < p.fit ? p.fit : most;
+    }
+    for (int i = 0; i < n && best.fit == 0; i++)
+      if (100 * plans[i].fit >= 93 * most) best = plans[i];
+    if (best.fit == 0) return cudaErrorInvalidConfiguration;
+  }
+  *out = best;
+  return cudaSuccess;
 }
 // launches `clusters` clusters of c blocks, with programmatic stream
 // serialization
@@ -1593,19 +1627,6 @@ cudaError_t launch_clusters(cudaStream_t s, void (*kern)(KArgs...), int clusters
   cfg.numAttrs = c > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
-// clusters above 8 blocks have to be allowed, once per kernel and device
-cudaError_t allow_large_clusters(const void* kern) {
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev)) return e;
-  static std::mutex mu;
-  static std::set<std::pair<const void*, int>> done;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done.count({kern, dev})) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) done.insert({kern, dev});
-  return e;
-}
-
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // what a forward call keeps between its two kernels
 size_t workspace_bytes(int dtype, int n, int vocab, int top) {
@@ -1697,19 +1718,15 @@ cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
   ws.z = reinterpret_cast<float*>(take(n * k * sizeof(float)));
   ws.ticket = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t)));
   const auto kern = step_kernel<T, ENTROPY>;
-  // a warp per segment
-  const int nseg = (L.vocab + kSeg - 1) / kSeg, c = (nseg + kWarps - 1) / kWarps, warps = (nseg + c - 1) / c;
-  const size_t smem = warps * kStageBytes<T>;
-  if (cudaError_t e = raise_smem_cap((const void*)kern, smem)) return e;
-  if (c > 8)
-    if (cudaError_t e = allow_large_clusters((const void*)kern)) return e;
-  const int fit = resident_clusters((const void*)kern, c, 32 * warps, smem), clusters = L.n < fit ? L.n : fit;
+  ClusterPlan plan;
+  if (cudaError_t e = cluster_plan((const void*)kern, (L.vocab + kSeg - 1) / kSeg, kStageBytes<T>, &plan)) return e;
+  const int clusters = L.n < plan.fit ? L.n : plan.fit;
   step_gather_kernel<T>
       <<<(L.n + kWarps - 1) / kWarps, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, ws, 2 * clusters);
   if (cudaError_t e = cudaGetLastError()) return e;
   T* y = static_cast<T*>(out);
-  if (cudaError_t e = launch_clusters(s, kern, clusters, c, 32 * warps, smem, L, temp, ws, o.stats, o.flags, y, out_ld,
-                                      1.0f))
+  if (cudaError_t e = launch_clusters(s, kern, clusters, plan.c, 32 * plan.warps, plan.warps * kStageBytes<T>, L, temp,
+                                      ws, o.stats, o.flags, y, out_ld, 1.0f))
     return e;
   const Launch launch{s, nullptr, nullptr, true};
   return launch_k(launch, step_rows_kernel<T, ENTROPY>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes, te, temp,
