@@ -19,6 +19,7 @@ There is no CPU fallback.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -112,6 +113,16 @@ def _new(logits, *shape):
     return logits.new_empty(shape, dtype=_F32)
 
 
+@functools.lru_cache(maxsize=256)
+def _scores_size(dtype, n, vocab, top):
+    return lib().det_scores_workspace(_DTYPES[dtype], n, vocab, top)
+
+
+@functools.lru_cache(maxsize=256)
+def _step_size(n, vocab, k):
+    return lib().det_step_workspace(n, vocab, k)
+
+
 def _workspace(logits, size):
     return logits.new_empty(size, dtype=torch.uint8), size
 
@@ -122,14 +133,14 @@ def token_scores(logits, tokens, top: int = 0) -> TokenScores:
     in the order of their ids."""
     n, vocab, ld = _logits(logits)
     tok = _on(tokens, logits, "tokens", (n,), _IDS)
+    if not 0 <= top <= min(vocab, 128):
+        raise ValueError("top must be in 0 .. 128 and at most the vocabulary")
     logprob, entropy, stats = _new(logits, n), _new(logits, n), _new(logits, n, 4)
     ids = lps = None
     if top:
-        if top < 0:
-            raise ValueError("top must not be negative")
         ids = logits.new_empty((n, top), dtype=torch.int32)
         lps = _new(logits, n, top)
-    work, size = _workspace(logits, lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, top))
+    work, size = _workspace(logits, _scores_size(logits.dtype, n, vocab, top))
     _call("det_token_scores_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
           _IDS[tokens.dtype], top, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
           ids.data_ptr() if top else None, lps.data_ptr() if top else None, None, work.data_ptr(), size)
@@ -161,7 +172,7 @@ def token_scores_step(logits, tokens, grad_logprob=None, grad_entropy=None, out=
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     logprob, entropy, stats = _new(logits, n), _new(logits, n), _new(logits, n, 4)
-    work, size = _workspace(logits, lib().det_step_workspace(n, vocab, 1))
+    work, size = _workspace(logits, _step_size(n, vocab, 1))
     _call("det_token_scores_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
           _IDS[tokens.dtype], gl, ge, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld,
           None, work.data_ptr(), size)
@@ -176,7 +187,7 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) 
     n, vocab, ld = _logits(logits)
     lists = _lists(teacher_ids, teacher_logits, logits, n)
     loss, stats = _new(logits, n), _new(logits, n, 4)
-    work, size = _workspace(logits, lib().det_scores_workspace(_DTYPES[logits.dtype], n, vocab, 0))
+    work, size = _workspace(logits, _scores_size(logits.dtype, n, vocab, 0))
     _call("det_distill_loss_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
           temperature, loss.data_ptr(), stats.data_ptr(), None, work.data_ptr(), size)
     return DistillLoss(loss, stats)
@@ -205,7 +216,7 @@ def distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperature: fl
     g = _vector(grad_loss, logits, "grad_loss", n)
     out, out_ld = _grad_out(logits, out, n, vocab)
     loss, stats = _new(logits, n), _new(logits, n, 4)
-    work, size = _workspace(logits, lib().det_step_workspace(n, vocab, lists[4]))
+    work, size = _workspace(logits, _step_size(n, vocab, lists[4]))
     _call("det_distill_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
           temperature, g, loss.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld, None, work.data_ptr(), size)
     return DistillLoss(loss, stats), out

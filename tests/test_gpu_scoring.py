@@ -610,8 +610,11 @@ def test_lists_of_wider_rows_and_of_one_row(env):
         sc.distill_loss(x, ids[:, 3:20], u[:, 3:20].contiguous())
     with pytest.raises(ValueError):
         sc.distill_loss(x.t(), ids, u)
-    with pytest.raises(D.DetError):
-        sc.token_scores(x, torch.zeros(6, dtype=torch.int64, device="cuda"), top=129)
+    for top in (129, -1):
+        with pytest.raises(ValueError):
+            sc.token_scores(x, torch.zeros(6, dtype=torch.int64, device="cuda"), top=top)
+    with pytest.raises(D.DetError):  # a gradient of nothing
+        sc.token_scores_step(x, torch.zeros(6, dtype=torch.int64, device="cuda"))
 
 
 @pytest.mark.parametrize("t", [1e-6, 1e-3, 1e3, 1e6])
