@@ -912,8 +912,9 @@ constexpr int kSegThreads = 256, kSegBlocks = 2;
 // and the parts are even however many rows there are.  A segment's sums and
 // its groups' maxima go to the caller's workspace.  In the second, a block per
 // row joins the row's segments and writes its results.  (One kernel with a
-// block or cluster per row lost 16 to 25% to uneven rounds of rows and to the
-// rows' ends: 119 us against 104 for 1,024 rows of 128,256 f32 logits.)
+// block or cluster per row loses to uneven rounds of rows and at the rows'
+// ends: 136 us against 122 for 1,024 rows of 128,256 f32 logits, with the same
+// arithmetic and the cache flushed before each.)
 //
 // The first kernel reads each logit once.  1,024 rows of 128,256 f32: 90 us,
 // 5.8 TB/s of 6.5 copied; of 151,936 bf16: 90 us, 3.5 TB/s.  The latter is
