@@ -940,10 +940,10 @@ __global__ void __launch_bounds__(kSegThreads, kSegBlocks)
   const int first = blockIdx.x * (kSegThreads / 32) + (threadIdx.x >> 5);
   int row = first / nseg, g = first % nseg;
   const int drow = all / nseg, dg = all % nseg;
-  if (row < L.n) stage_issue<T>(stage, at_row(row), g, V);
-  pdl_trigger();
   const float c = fdiv(kLog2e, temp);
   const uint32_t table = kExpTable[l];
+  pdl_enter();
+  if (row < L.n) stage_issue<T>(stage, at_row(row), g, V);
   while (row < L.n) {
     uint4 v[G::NV];
     stage_take<T>(stage, misaligned(at_row(row)), v);
@@ -1139,11 +1139,13 @@ __global__ void __launch_bounds__(kThreads, 3)
     }
   };
   const int w = threadIdx.x >> 5;
+  const float c = fdiv(kLog2e, temp);
+  const uint32_t table = kExpTable[l];
   uint4 cur[U];
+  pdl_enter();
   if (q0 + w * kGradRun < q1) fetch(q0 + w * kGradRun, cur);
   const float* st = in.stats + (size_t)row * 4;
-  const float m = st[0], s = st[1], c = fdiv(kLog2e, temp);
-  const uint32_t table = kExpTable[l];
+  const float m = st[0], s = st[1];
   RowGrad r;
   int id;
   float add;
@@ -1302,6 +1304,7 @@ __global__ void __launch_bounds__(kThreads)
     step_gather_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, StepWork ws,
                        uint32_t first) {
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), l = threadIdx.x & 31, V = L.vocab;
+  pdl_wait();
   if (row >= L.n) return;
   if (row == 0 && l == 0) *ws.ticket = first;
   const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
@@ -1677,9 +1680,10 @@ cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int 
   Workspace ws;
   ws.seg = static_cast<float4*>(workspace);
   ws.gmax = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256(L.n * nseg * sizeof(float4)));
-  segments<<<(unsigned)(blocks < fit ? blocks : fit), kSegThreads, smem, s>>>(L, temp, ws, 1.0f);
-  if (cudaError_t e = cudaGetLastError()) return e;
   const Launch launch{s, nullptr, nullptr, true};
+  if (cudaError_t e = launch_k(launch, segments, dim3((unsigned)(blocks < fit ? blocks : fit)), dim3(kSegThreads), smem,
+                               L, temp, ws, 1.0f))
+    return e;
   return launch_k(launch, rows_kernel<T, TOP>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes,
                   te, temp, ws, loss, o, 1.0f);
 }
@@ -1710,10 +1714,12 @@ cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
   // and less than a run of each warp where SMs would be without a block
   while (per > kGradRun && (long long)L.n * ((nvec + per - 1) / per) < device_sms()) per /= 2;
   const int blocks = (nvec + per - 1) / per;
+  const Launch launch{s, nullptr, nullptr, true};
   for (int r = 0; r < L.n; r += 65535) {
-    grad_kernel<T, ENTROPY><<<dim3(blocks, L.n - r < 65535 ? L.n - r : 65535), kThreads, 0, s>>>(
-        L, r, per, tokens, id_bytes, te, temp, in, static_cast<T*>(out), out_ld, 1.0f);
-    if (cudaError_t e = cudaGetLastError()) return e;
+    if (cudaError_t e = launch_k(launch, grad_kernel<T, ENTROPY>, dim3(blocks, L.n - r < 65535 ? L.n - r : 65535),
+                                 dim3(kThreads), 0, L, r, per, tokens, id_bytes, te, temp, in, static_cast<T*>(out),
+                                 out_ld, 1.0f))
+      return e;
   }
   return cudaSuccess;
 }
@@ -1748,14 +1754,14 @@ cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
   ClusterPlan plan;
   if (cudaError_t e = cluster_plan((const void*)kern, (L.vocab + kSeg - 1) / kSeg, kStageBytes<T>, &plan)) return e;
   const int clusters = L.n < plan.fit ? L.n : plan.fit;
-  step_gather_kernel<T>
-      <<<(L.n + kWarps - 1) / kWarps, kThreads, 0, s>>>(L, tokens, id_bytes, te, temp, in, ws, 2 * clusters);
-  if (cudaError_t e = cudaGetLastError()) return e;
+  const Launch launch{s, nullptr, nullptr, true};
+  if (cudaError_t e = launch_k(launch, step_gather_kernel<T>, dim3((L.n + kWarps - 1) / kWarps), dim3(kThreads), 0, L,
+                               tokens, id_bytes, te, temp, in, ws, 2 * clusters))
+    return e;
   T* y = static_cast<T*>(out);
   if (cudaError_t e = launch_clusters(s, kern, clusters, plan.c, 32 * plan.warps, plan.warps * kStageBytes<T>, L, temp,
                                       ws, o.stats, o.flags, y, out_ld, 1.0f))
     return e;
-  const Launch launch{s, nullptr, nullptr, true};
   return launch_k(launch, step_rows_kernel<T, ENTROPY>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes, te, temp,
                   in, ws, loss, o, y, out_ld, 1.0f);
 }
