@@ -1374,15 +1374,17 @@ DI bool bar_done(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// waits for the barrier's phase, a second at most
+// waits for the barrier's phase, a second at most (and 4,096 tries at least, as
+// the clock runs on while the GPU does something else)
 DI bool bar_wait(uint32_t bar, uint32_t parity) {
   if (bar_done(bar, parity)) return true;
   unsigned long long t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  int tries = 0;
   do {
     if (bar_done(bar, parity)) return true;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  } while (t - t0 < 1000000000ull);
+  } while (++tries < 4096 || t - t0 < 1000000000ull);
   return false;
 }
 template <typename T, bool ENTROPY>
