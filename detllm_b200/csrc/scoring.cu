@@ -265,18 +265,23 @@ DI uint4 pack_vec(const float* v) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// The vector at entry `at` of a row that nothing writes meanwhile; what is past
-// the row's end is -inf.  Only 16-byte granules that lie in the row as a whole
+template <bool RO>
+DI uint4 load16(const uint4* p) {
+  if constexpr (RO) return __ldg(p);
+  else return *p;
+}
+// The vector at entry `at` of a row (RO: that nothing writes while the kernel
+// runs); what is past the row's end is -inf.  Only 16-byte granules that lie in the row as a whole
 // are loaded as such: a row that starts `mis` entries into a granule takes two
 // of them.
-template <typename T>
-DI uint4 row_vec(const T* __restrict__ row, int at, int V, int mis) {
+template <typename T, bool RO = true>
+DI uint4 row_vec(const T* row, int at, int V, int mis) {
   constexpr int VEC = Seg<T>::VEC;
   const T* p = row + at;
-  if (mis == 0 && at + VEC <= V) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (mis == 0 && at + VEC <= V) return load16<RO>(reinterpret_cast<const uint4*>(p));
   if (mis != 0 && at >= mis && at - mis + 2 * VEC <= V) {
     const uint4* q = reinterpret_cast<const uint4*>(p - mis);
-    return shifted(__ldg(q), __ldg(q + 1), mis * (int)sizeof(T));
+    return shifted(load16<RO>(q), load16<RO>(q + 1), mis * (int)sizeof(T));
   }
   float v[VEC];
 #pragma unroll
@@ -561,12 +566,13 @@ struct Teacher {
 };
 
 // ---- the teacher's list of one row ---------------------------------------------
+constexpr int kListWarps = 16;  // of a block that takes a row's list, at most
 struct ListShared {
-  float max[kWarps], sum[kWarps];
-  int bad[kWarps], some[kWarps];
+  float max[kListWarps], sum[kListWarps];
+  int bad[kListWarps], some[kListWarps];
   int id[DET_MAX_TOP];
   float q[DET_MAX_TOP];
-  double term[kWarps];
+  double term[kListWarps];
 };
 struct ListEntry {
   int id;         // -1: not a valid entry
@@ -1337,6 +1343,39 @@ DI RowGrad row_grad(float a_g, float a_h, bool zero, const RowStats& r, float c)
   const float a = a_h == 0.0f ? a_g : fadd(a_g, fmul(a_h, fdiv(r.s1, r.s)));
   return {-r.m, c, fmul(a, inv_s), fmul(fmul(-a_h, kLn2), inv_s), zero || r.empty};
 }
+// The gradient of segment g of a row with maximum m to y, from its logits
+// (ENTROPY) or from their exponentials under the segment's maximum.
+template <typename T, bool ENTROPY>
+DI void grad_segment(const uint4 (&raw)[Seg<T>::NV], const float* v, float m_seg, float m, const RowGrad& rg, float c,
+                     uint32_t table, float one_, T* y, int g, int V) {
+  using G = Seg<T>;
+  const f2 one = pk(one_, one_), cc = pk(c, c);
+  const float y_seg = segment_y(m_seg, m, c);
+  const float f = fmul(un(exp2_warp<true>(pk(y_seg, y_seg), table, one).e).x, rg.as);
+  // vector i of the segment's gradient
+  auto vec = [&](int i) {
+    constexpr int VEC = G::VEC;
+    if (rg.zero) return make_uint4(0, 0, 0, 0);
+    float x[VEC];
+    f2 dx[VEC / 2];
+    if constexpr (ENTROPY) add_vec<T>(raw[i], rg.base, dx);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      f2 d;
+      if constexpr (ENTROPY) {
+        const Exp2 ex = exp2_warp<true>(mul2(dx[j / 2], cc), table, one);
+        d = grad2<true>(ex.e, ex.y, rg, one);
+      } else {
+        d = mul2(pk(v[i * VEC + j], v[i * VEC + j + 1]), pk(f, f));
+      }
+      const float2 dv = un(d);
+      x[j] = dv.x;
+      x[j + 1] = dv.y;
+    }
+    return pack_vec<T>(x);
+  };
+  store_segment<T>(y, g, V, misaligned(y), vec);
+}
 DI uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -1467,33 +1506,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         float* st = stats + (size_t)row * 4;
         st[0] = r.m, st[1] = r.s, st[2] = r.s1;
       }
-      const f2 one = pk(one_, one_), cc = pk(c, c);
-      const float y_seg = segment_y(m_seg, r.m, c);
-      const float f = fmul(un(exp2_warp<true>(pk(y_seg, y_seg), table, one).e).x, rg.as);
-      // vector i of the segment's gradient
-      auto vec = [&](int i) {
-        constexpr int VEC = G::VEC;
-        if (rg.zero) return make_uint4(0, 0, 0, 0);
-        float x[VEC];
-        f2 dx[VEC / 2];
-        if constexpr (ENTROPY) add_vec<T>(raw[i], rg.base, dx);
-#pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          f2 d;
-          if constexpr (ENTROPY) {
-            const Exp2 ex = exp2_warp<true>(mul2(dx[j / 2], cc), table, one);
-            d = grad2<true>(ex.e, ex.y, rg, one);
-          } else {
-            d = mul2(pk(v[i * VEC + j], v[i * VEC + j + 1]), pk(f, f));
-          }
-          const float2 dv = un(d);
-          x[j] = dv.x;
-          x[j + 1] = dv.y;
-        }
-        return pack_vec<T>(x);
-      };
-      T* y = out + (size_t)row * out_ld;
-      store_segment<T>(y, g, V, misaligned(y), vec);
+      grad_segment<T, ENTROPY>(raw, v, m_seg, r.m, rg, c, table, one_, out + (size_t)row * out_ld, g, V);
       row = next;
       next = there ? drawn : L.n;
     }
@@ -1550,6 +1563,107 @@ __global__ void __launch_bounds__(kRowThreads)
   if (loss) {
     const float v = list_loss(e, logq, z, r, log_s, temp, list);
     if (threadIdx.x == 0) loss[row] = v;
+  }
+}
+
+// Rows of few segments, few enough that an SM has them all at once: scores
+// without a top list, or scores and gradient, in one kernel with a block per row
+// and a warp per segment.  All of a row is read before any of its gradient is
+// written.  Bound by latency: one load, the sums, the list's sums and a 64-bit
+// logarithm follow one another.  What it saves are launches, of two or three.
+// bf16, us per call, in a stream and in a graph, against the kernels above:
+//                                   148 x 2,000          148 x 32,000
+//   scores                      13.7 -> 11.1, 5.0 -> 3.6   13.6 -> 11.2, 6.4 -> 5.1
+//   distillation loss           12.6 -> 10.2, 5.3 -> 6.3   13.3 -> 11.4, 7.0 -> 7.6
+//   scores and gradient         15.9 -> 11.5, 8.6 -> 5.6   15.7 -> 11.4, 13.6 -> 7.2
+//   entropy's gradient too      15.8 -> 11.6, 11.0 -> 7.0  18.8 -> 11.7, 17.6 -> 8.8
+//   distillation and gradient   15.2 -> 10.9, 10.3 -> 8.3  15.5 -> 11.0, 14.5 -> 10.0
+// With more rows than that it loses: 592 x 32,000 31.5 -> 38.2 for the last,
+// 17.0 -> 18.6 for the first.  With a top list the block's warps are too few for
+// the list: 9 -> 11 us for 1 x 2,000, 9 -> 16 for 1 x 32,000.
+enum { kScores, kGrad, kGradEntropy };
+constexpr int kSmallSegs = kListWarps;
+template <typename T, int MODE>
+__global__ void __launch_bounds__(32 * kSmallSegs)
+    small_rows_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, float* loss,
+                      ScoreOut o, T* out, unsigned long long out_ld, float one) {
+  using G = Seg<T>;
+  constexpr bool ENTROPY = MODE == kGradEntropy;
+  __shared__ ListShared list;
+  __shared__ float4 seg[kSmallSegs];
+  const int row = blockIdx.x, V = L.vocab, g = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const int nseg = (V + kSeg - 1) / kSeg;
+  const float c = fdiv(kLog2e, temp), nan = __int_as_float(0x7fffffff);
+  const uint32_t table = kExpTable[l];
+  pdl_enter();
+  const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
+  const int mis = misaligned(x);
+  uint4 raw[G::NV];
+  float v[MODE == kGrad ? kPerLane : 1], m_seg = -INFINITY;
+  if (g < nseg) {
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) raw[i] = row_vec<T, MODE == kScores>(x, g * kSeg + (32 * i + l) * G::VEC, V, mis);
+    Range<T> range;
+#pragma unroll
+    for (int i = 0; i < G::NV; i++) range.take(raw[i]);
+    m_seg = redux_max(range.high());
+    const float s =
+        segment_sums<T, MODE == kGrad>(raw, V - g * kSeg, m_seg, redux_min(range.low()), c, table, one, v);
+    const float w = __shfl_sync(kFull, s, 16);
+    if (l == 0) seg[g] = make_float4(m_seg, s, w, 0.0f);
+  }
+  // the row's own tokens, and the gradient's coefficients (as in StepWork)
+  ListEntry e;
+  double logq = 0.0;
+  long long t = -1;
+  int id = -1;
+  float z = 0.0f, share = 0.0f, a_g = 0.0f, a_h = 0.0f;
+  bool zero = false;
+  if (te.k) {
+    e = teacher_entry(te, row, V, c, table, one, list);
+    if (e.id >= 0) z = to_f32(x[e.id]);
+    logq = list_logq(e, temp);
+    if constexpr (MODE != kScores) {
+      ListEntry f = e;
+      share = list_share(f, te.k, list);
+      id = f.id;
+      a_g = e.bad ? nan : fdiv(in.g[row], temp);
+      zero = !e.some && !e.bad;
+    }
+  } else {
+    if (tokens) t = load_id(tokens, id_bytes, row);
+    if (t >= 0 && t < V) z = to_f32(x[t]);
+    if constexpr (MODE != kScores) {
+      if (threadIdx.x == 0 && t >= 0 && t < V) id = (int)t;
+      a_g = -(!in.g || t < 0 ? 0.0f : t >= V ? nan : in.g[row]);
+      a_h = in.gh ? in.gh[row] : 0.0f;
+    }
+  }
+  __syncthreads();  // the sums are there, and the row is read
+  const RowStats r = finish_row(join_segments<true>(
+      [&](int i) {
+        const float4 f = seg[i];
+        return Sums{f.x, f.y, f.z};
+      },
+      nseg, c, table, one));
+  if constexpr (MODE != kScores) {
+    const RowGrad rg = row_grad(a_g, a_h, zero, r, c);
+    T* y = out + (size_t)row * out_ld;
+    if (g < nseg) grad_segment<T, ENTROPY>(raw, v, m_seg, r.m, rg, c, table, one, y, g, V);
+    __syncthreads();  // behind the rest of the row's gradient:
+    if (id >= 0 && !rg.zero)
+      y[id] = from_f32<T>(fadd(grad1<ENTROPY>(z, rg, one), te.k ? fmul(-a_g, share) : -a_g));
+  }
+  const double log_s = threadIdx.x < max(1, te.k) ? log_sum(r) : 0.0;
+  if (threadIdx.x == 0) {
+    if (o.stats) write_stats(o.stats, row, r, log_s);
+    if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+    if ((te.k ? e.bad : t >= V) && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
+    if (!te.k) write_scores(o, row, V, r, log_s, t, z);
+  }
+  if (te.k) {
+    const float sum = list_loss(e, logq, z, r, log_s, temp, list);
+    if (threadIdx.x == 0) loss[row] = sum;
   }
 }
 
@@ -1660,6 +1774,21 @@ cudaError_t launch_clusters(cudaStream_t s, void (*kern)(KArgs...), int clusters
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+// Whether small_rows_kernel takes the rows: all of them at once, at 16 warps per
+// SM.
+int small_warps(int nseg) { return nseg < 4 ? 4 : nseg; }  // a thread per list entry
+bool small_rows(int n, int vocab) {
+  const int nseg = (vocab + kSeg - 1) / kSeg;
+  return nseg <= kSmallSegs && n <= device_sms() * (16 / small_warps(nseg));
+}
+int forward_launches(int n, int vocab, int top) { return !top && small_rows(n, vocab) ? 1 : 2; }
+template <typename T, int MODE>
+cudaError_t small_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
+                     const GradIn& in, float* loss, const ScoreOut& o, void* out, unsigned long long out_ld) {
+  const int warps = small_warps((L.vocab + kSeg - 1) / kSeg);
+  return launch_k(Launch{s, nullptr, nullptr, true}, small_rows_kernel<T, MODE>, dim3(L.n), dim3(32 * warps), 0, L,
+                  tokens, id_bytes, te, temp, in, loss, o, static_cast<T*>(out), out_ld, 1.0f);
+}
 // what a forward call keeps between its two kernels
 size_t workspace_bytes(int dtype, int n, int vocab, int top) {
   const size_t nseg = (vocab + kSeg - 1) / kSeg, vec = dtype == DET_DTYPE_F32 ? 4 : 8;
@@ -1669,6 +1798,8 @@ size_t workspace_bytes(int dtype, int n, int vocab, int top) {
 template <typename T, bool TOP>
 cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te,
                        float temp, void* workspace, float* loss, const ScoreOut& o) {
+  if (!TOP && small_rows(L.n, L.vocab))
+    return small_as<T, kScores>(s, L, o.logprob ? tokens : nullptr, id_bytes, te, temp, GradIn{}, loss, o, nullptr, 0);
   const int lg = TOP ? group_lanes_log2(L.vocab, o.top, Seg<T>::VEC) : -1;
   const auto segments = lg < 0    ? segments_kernel<T, -1>
                         : lg == 0 ? segments_kernel<T, 0>
@@ -1741,6 +1872,8 @@ template <typename T, bool ENTROPY>
 cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
                     const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
                     unsigned long long out_ld) {
+  if (small_rows(L.n, L.vocab))
+    return small_as<T, ENTROPY ? kGradEntropy : kGrad>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld);
   const size_t n = L.n, k = te.k ? te.k : 1;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   auto take = [&](size_t bytes) {
@@ -1843,7 +1976,7 @@ cudaError_t launch_token_scores(const Launch& L, const float* logits, int V, con
                                 int32_t* top_ids, float* top_logprobs, void* workspace) {
   const Logits x{logits, rows, (unsigned long long)V, n, V};
   const ScoreOut o{logprob, entropy, nullptr, top_ids, top_logprobs, top, L.err};
-  if (L.launches) *L.launches += 2;
+  if (L.launches) *L.launches += forward_launches(n, V, top);
   return launch_forward(L.stream, DET_DTYPE_F32, x, tokens, 4, kNoTeacher, 1.0f, workspace, nullptr, o);
 }
 cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, const uint32_t* rows, int n,
@@ -1852,7 +1985,7 @@ cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, con
   const Logits x{logits, rows, (unsigned long long)V, n, V};
   const Teacher te{ids, teacher, (unsigned long long)k, 4, DET_DTYPE_F32, k};
   const ScoreOut o{nullptr, nullptr, nullptr, nullptr, nullptr, 0, L.err};
-  if (L.launches) *L.launches += 2;
+  if (L.launches) *L.launches += forward_launches(n, V, 0);
   return launch_forward(L.stream, DET_DTYPE_F32, x, nullptr, 4, te, temperature, workspace, loss, o);
 }
 

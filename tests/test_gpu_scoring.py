@@ -431,6 +431,35 @@ def test_a_row_alone_is_a_row_in_a_batch(env, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1, 300, 2049, 9001, 16385, 32768, 32769])
+def test_few_rows_and_one_more(env, vocab, dtype):
+    """One kernel takes as many short rows as the device holds at once, other
+    kernels one row more: the same bits."""
+    _, torch, sc = env
+    warps = max(4, -(-vocab // 2048))
+    most = 16 // warps * torch.cuda.get_device_properties(0).multi_processor_count if warps <= 16 else 5
+    x, tokens, g = make(torch, most + 1, vocab, getattr(torch, dtype), vocab, 3, 1, True)
+    x[2] = float("nan")
+    x[3, 0] = INF
+    one = torch.randn(most + 1, generator=g, device="cuda")
+    k = min(vocab, 33)
+    ids, u = lists(torch, x, k, g, torch.float32, "twice")
+
+    def calls(s):
+        y = x.clone()[s]
+        yield from sc.token_scores(x[s], tokens[s])[:3]
+        yield from sc.distill_loss(x[s], ids[s], u[s], 0.7)
+        for entropy in (None, one[s]):
+            a, b = sc.token_scores_step(x[s], tokens[s], one[s], entropy)
+            yield from (*a[:3], b)
+        a, b = sc.distill_step(y, ids[s], u[s], one[s], 0.7, out=y)
+        yield from (*a, b)
+
+    for a, b in zip(calls(slice(0, most)), calls(slice(0, most + 1)), strict=True):
+        assert torch.equal(torch.nan_to_num(a.float(), nan=1e30), torch.nan_to_num(b[:most].float(), nan=1e30))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,vocab,pad,shift", [(5, 1003, 9, 1), (3, 40001, 1, 0), (200, 32000, 8, 0), (4, 151936, 5, 3)])
 def test_gradient_in_place_and_beside(env, n, vocab, pad, shift, dtype):
     """Over the logits, into rows of another stride, and side by side with
