@@ -17,9 +17,10 @@
 // is part of (the gradients of the step kernel and of the gradient kernel are
 // scaled in another order and may differ in their last bits).  Sums and sums'
 // joins are f32, logarithms and what is made of them 64 bits, and gradients
-// are rounded once to the logits' type.  A row is cut into segments of 2,048 entries; a warp takes a segment, its
-// lane l the entries of 16-byte vectors l, l + 32, ... of it, and sums are
-// relative to the segment's own maximum until the segments are joined.
+// are rounded once to the logits' type.  A row is cut into segments of 2,048
+// entries; a warp takes a segment, its lane l the entries of 16-byte vectors l,
+// l + 32, ... of it, and sums are relative to the segment's own maximum until
+// the segments are joined.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -271,9 +272,9 @@ DI uint4 load16(const uint4* p) {
   else return *p;
 }
 // The vector at entry `at` of a row (RO: that nothing writes while the kernel
-// runs); what is past the row's end is -inf.  Only 16-byte granules that lie in the row as a whole
-// are loaded as such: a row that starts `mis` entries into a granule takes two
-// of them.
+// runs); what is past the row's end is -inf.  Only 16-byte granules that lie in
+// the row as a whole are loaded as such: a row that starts `mis` entries into a
+// granule takes two of them.
 template <typename T, bool RO = true>
 DI uint4 row_vec(const T* row, int at, int V, int mis) {
   constexpr int VEC = Seg<T>::VEC;
