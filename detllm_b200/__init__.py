@@ -121,6 +121,7 @@ def lib():
             "det_distill_step_device": (I, [P, I, U32, U32, U64, P, I, P, I, U32, U64, F32, P, P, P, P, U64, P, P, SZ, P]),
             "det_tp_exchange_timeout_selftest": (I, [I]),
             "det_q6k_pipeline_timeout_selftest": (I, [I]),
+            "det_step_timeout_selftest": (I, [I]),
             "det_add_latency_cycles": (I, [I, C.POINTER(C.c_double)]),
         }
         for name, (res, args) in sig.items():

@@ -1304,7 +1304,7 @@ DI void store_segment(T* y, int g, int V, int my, F vec) {
 struct StepWork {
   float4* coef;      // per row: of the loss over T, or of minus logprob; of the entropy; 1 where all is zeros
   float* z;          // per row and entry: the logit at its token
-  uint32_t* ticket;  // rows drawn
+  uint32_t* ticket;  // [0]: rows drawn; [1]: not 0 once a wait has run out
 };
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -1313,7 +1313,7 @@ __global__ void __launch_bounds__(kThreads)
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), l = threadIdx.x & 31, V = L.vocab;
   pdl_wait();
   if (row >= L.n) return;
-  if (row == 0 && l == 0) *ws.ticket = first;
+  if (row == 0 && l == 0) ws.ticket[0] = first, ws.ticket[1] = 0;
   const T* x = static_cast<const T*>(L.x) + (size_t)row * L.ld;
   const float nan = __int_as_float(0x7fffffff);
   if (te.k) {
@@ -1414,9 +1414,9 @@ DI bool bar_done(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// waits for the barrier's phase, a second at most (and 4,096 tries at least, as
+// waits for the barrier's phase, `limit_ns` at most (and min_tries at least, as
 // the clock runs on while the GPU does something else)
-DI bool bar_wait(uint32_t bar, uint32_t parity) {
+DI bool bar_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns, int min_tries) {
   if (bar_done(bar, parity)) return true;
   unsigned long long t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
@@ -1424,13 +1424,19 @@ DI bool bar_wait(uint32_t bar, uint32_t parity) {
   do {
     if (bar_done(bar, parity)) return true;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  } while (++tries < 4096 || t - t0 < 1000000000ull);
+  } while (++tries < min_tries || t - t0 < limit_ns);
   return false;
 }
-template <typename T, bool ENTROPY>
+// SELFTEST: waits of 20 ms, one of which runs out: the last block of the first
+// cluster expects one arrival more than comes on its second barrier.
+template <bool SELFTEST>
+struct StepWait {
+  static constexpr unsigned long long ns = SELFTEST ? 20000000ull : 1000000000ull;
+  static constexpr int tries = SELFTEST ? 16 : 4096;
+};
+template <typename T, bool ENTROPY, bool SELFTEST = false>
 __global__ void __launch_bounds__(kThreads, 2)
-    step_kernel(Logits L, float temp, StepWork ws, float* stats, uint32_t* flags, T* out, unsigned long long out_ld,
-                float one_) {
+    step_kernel(Logits L, float temp, StepWork ws, float* stats, T* out, unsigned long long out_ld, float one_) {
   using G = Seg<T>;
   __shared__ float4 seg[2][kMaxSegs];
   __shared__ __align__(8) unsigned long long bars[2];
@@ -1449,8 +1455,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t table = kExpTable[l], bar = shared_at(bars);
   if (threadIdx.x == 0) {
     // a lone block's warps arrive themselves
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\nmbarrier.init.shared::cta.b64 [%0 + 8], %1;" ::"r"(bar),
-                 "r"(size > 1 ? 1 : nseg)
+    const int count = size > 1 ? 1 : nseg;
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\nmbarrier.init.shared::cta.b64 [%0 + 8], %2;" ::"r"(bar),
+                 "r"(count), "r"(SELFTEST && blockIdx.x == size - 1 ? count + 1 : count)
                  : "memory");
     if (size > 1) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1489,28 +1496,31 @@ __global__ void __launch_bounds__(kThreads, 2)
         asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar + 8 * half) : "memory");
       }
       // The wait ends: the other warps run, and send what this one waits for
-      // without waiting for this row.  Should it not, the row is given up as
-      // NaN and the warp stops after the next.
-      const bool there = __all_sync(kFull, bar_wait(bar + 8 * half, (turn >> 1) & 1));
-      if (!there && l == 0 && flags) atomicOr(flags, (uint32_t)DET_SCORE_TIMEOUT);
+      // without waiting for this row.  Should it run out, the warp says so and
+      // leaves behind this row, without sending again, so the cluster's other
+      // warps' waits run out too and the rows it had drawn stay undone: the next
+      // kernel makes all of the call's results NaN.
+      using Wait = StepWait<SELFTEST>;
+      const bool there = __all_sync(kFull, bar_wait(bar + 8 * half, (turn >> 1) & 1, Wait::ns, Wait::tries));
+      if (!there && l == 0) atomicOr(ws.ticket + 1, 1u);
       auto sums_of = [&](int i) {
         const float4 f = seg[half][i];
         return Sums{f.x, f.y, f.z};
       };
       // the sum of 2^y y is for the entropy's gradient, and for one warp to write
-      RowStats r = finish_row(ENTROPY || g == 0 ? join_segments<true>(sums_of, nseg, c, table, one_)
-                                                : join_segments<false>(sums_of, nseg, c, table, one_));
+      const RowStats r = finish_row(ENTROPY || g == 0 ? join_segments<true>(sums_of, nseg, c, table, one_)
+                                                      : join_segments<false>(sums_of, nseg, c, table, one_));
       const int drawn = (int)__float_as_uint(seg[half][0].w);
-      if (!there) r.m = r.s = r.s1 = __int_as_float(0x7fffffff), r.empty = false;
       const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
       if (g == 0 && l == 0) {
         float* st = stats + (size_t)row * 4;
         st[0] = r.m, st[1] = r.s, st[2] = r.s1;
       }
       grad_segment<T, ENTROPY>(raw, v, m_seg, r.m, rg, c, table, one_, out + (size_t)row * out_ld, g, V);
-      row = next;
-      next = there ? drawn : L.n;
+      row = there ? next : L.n;
+      next = drawn;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // of a warp that left early
   }
   // nobody leaves while another block may still send to it
   if (size > 1) {
@@ -1545,25 +1555,32 @@ __global__ void __launch_bounds__(kRowThreads)
   pdl_wait();
   const float z = own >= 0 ? ws.z[(size_t)row * (loss ? te.k : 1) + threadIdx.x] : 0.0f;
   const float4 coef = ws.coef[row];
-  const float* st = o.stats + (size_t)row * 4;
+  // a wait ran out: whichever rows were not finished, all of them are NaN
+  const bool lost = ws.ticket[1] != 0;
+  const float nan = __int_as_float(0x7fffffff);
+  float* st = o.stats + (size_t)row * 4;
+  T* y = out + (size_t)row * out_ld;
   RowStats r;
-  r.m = st[0], r.s = st[1], r.s1 = st[2];
+  r.m = lost ? nan : st[0], r.s = lost ? nan : st[1], r.s1 = lost ? nan : st[2];
   r.bad = !(r.m == r.m), r.empty = r.m == -INFINITY;
   const double log_s = log_sum(r);
   const RowGrad rg = row_grad(coef.x, coef.y, coef.z != 0.0f, r, c);
-  if (id >= 0 && !rg.zero) {
+  if (lost) {
+    for (int j = threadIdx.x; j < V; j += kRowThreads) y[j] = from_f32<T>(nan);
+  } else if (id >= 0 && !rg.zero) {
     const float add = loss ? fmul(-coef.x, share) : -coef.x;
-    out[(size_t)row * out_ld + id] = from_f32<T>(fadd(grad1<ENTROPY>(z, rg, one), add));
+    y[id] = from_f32<T>(fadd(grad1<ENTROPY>(z, rg, one), add));
   }
   if (threadIdx.x == 0) {
-    o.stats[(size_t)row * 4 + 3] = (float)log_s;
-    if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_NONFINITE);
+    st[3] = (float)log_s;
+    if (lost) st[0] = st[1] = st[2] = nan;
+    if (r.bad && o.flags) atomicOr(o.flags, (uint32_t)(lost ? DET_SCORE_TIMEOUT : DET_SCORE_NONFINITE));
     if ((loss ? e.bad : t >= V) && o.flags) atomicOr(o.flags, (uint32_t)DET_SCORE_BAD_TOKEN);
     if (!loss) write_scores(o, row, V, r, log_s, t, z);
   }
   if (loss) {
     const float v = list_loss(e, logq, z, r, log_s, temp, list);
-    if (threadIdx.x == 0) loss[row] = v;
+    if (threadIdx.x == 0) loss[row] = lost ? nan : v;
   }
 }
 
@@ -1867,14 +1884,13 @@ cudaError_t launch_grad(cudaStream_t s, int dtype, const Logits& L, const void* 
 }
 
 size_t step_workspace_bytes(size_t n, int k) {
-  return align256(n * sizeof(float4)) + align256(n * k * sizeof(float)) + align256(sizeof(uint32_t));
+  return align256(n * sizeof(float4)) + align256(n * k * sizeof(float)) + align256(2 * sizeof(uint32_t));
 }
-template <typename T, bool ENTROPY>
-cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
-                    const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
-                    unsigned long long out_ld) {
-  if (small_rows(L.n, L.vocab))
-    return small_as<T, ENTROPY ? kGradEntropy : kGrad>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld);
+// the three kernels; `most`: clusters at most
+template <typename T, bool ENTROPY, bool SELFTEST = false>
+cudaError_t clusters_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
+                        const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
+                        unsigned long long out_ld, int most) {
   const size_t n = L.n, k = te.k ? te.k : 1;
   uint8_t* at = static_cast<uint8_t*>(workspace);
   auto take = [&](size_t bytes) {
@@ -1885,21 +1901,29 @@ cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
   StepWork ws;
   ws.coef = reinterpret_cast<float4*>(take(n * sizeof(float4)));
   ws.z = reinterpret_cast<float*>(take(n * k * sizeof(float)));
-  ws.ticket = reinterpret_cast<uint32_t*>(take(sizeof(uint32_t)));
-  const auto kern = step_kernel<T, ENTROPY>;
+  ws.ticket = reinterpret_cast<uint32_t*>(take(2 * sizeof(uint32_t)));
+  const auto kern = step_kernel<T, ENTROPY, SELFTEST>;
   ClusterPlan plan;
   if (cudaError_t e = cluster_plan((const void*)kern, (L.vocab + kSeg - 1) / kSeg, kStageBytes<T>, &plan)) return e;
-  const int clusters = L.n < plan.fit ? L.n : plan.fit;
+  const int fit = plan.fit < most ? plan.fit : most, clusters = L.n < fit ? L.n : fit;
   const Launch launch{s, nullptr, nullptr, true};
   if (cudaError_t e = launch_k(launch, step_gather_kernel<T>, dim3((L.n + kWarps - 1) / kWarps), dim3(kThreads), 0, L,
                                tokens, id_bytes, te, temp, in, ws, 2 * clusters))
     return e;
   T* y = static_cast<T*>(out);
   if (cudaError_t e = launch_clusters(s, kern, clusters, plan.c, 32 * plan.warps, plan.warps * kStageBytes<T>, L, temp,
-                                      ws, o.stats, o.flags, y, out_ld, 1.0f))
+                                      ws, o.stats, y, out_ld, 1.0f))
     return e;
   return launch_k(launch, step_rows_kernel<T, ENTROPY>, dim3(L.n), dim3(kRowThreads), 0, L, tokens, id_bytes, te, temp,
                   in, ws, loss, o, y, out_ld, 1.0f);
+}
+template <typename T, bool ENTROPY>
+cudaError_t step_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
+                    const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
+                    unsigned long long out_ld) {
+  if (small_rows(L.n, L.vocab))
+    return small_as<T, ENTROPY ? kGradEntropy : kGrad>(s, L, tokens, id_bytes, te, temp, in, loss, o, out, out_ld);
+  return clusters_as<T, ENTROPY>(s, L, tokens, id_bytes, te, temp, in, workspace, loss, o, out, out_ld, L.n);
 }
 cudaError_t launch_step(cudaStream_t s, int dtype, const Logits& L, const void* tokens, int id_bytes,
                         const Teacher& te, float temp, const GradIn& in, void* workspace, float* loss,
@@ -1992,6 +2016,56 @@ cudaError_t launch_distill_loss(const Launch& L, const float* logits, int V, con
 
 size_t scores_workspace_bytes(int n, int V, int top) { return workspace_bytes(DET_DTYPE_F32, n, V, top); }
 
+// One run of the step on zero logits in rows of `vocab`, with a list of k ids or
+// (k = 0) with tokens, in two clusters that take several rows each; everything
+// it writes to is 0 before.  *all, *none: are all of its results NaN, none of
+// them; *flags: what it set.
+template <bool SELFTEST>
+cudaError_t step_selftest_run(int vocab, int k, bool* all, bool* none, uint32_t* flags) {
+  using T = __nv_bfloat16;
+  constexpr int n = 12, kIds = 2;
+  // logits | gradient | ids | f32: ones (the gradients of the results) | teacher | results, stats | flags | workspace
+  const size_t row_bytes = align256((size_t)n * vocab * sizeof(T)), small = 4096;
+  const size_t bytes = 2 * row_bytes + 5 * small + step_workspace_bytes(n, kIds);
+  uint8_t* mem = nullptr;
+  if (cudaError_t e = cudaMalloc(&mem, bytes)) return e;
+  T* grad = reinterpret_cast<T*>(mem + row_bytes);
+  int32_t* ids = reinterpret_cast<int32_t*>(mem + 2 * row_bytes);
+  float* ones = reinterpret_cast<float*>(mem + 2 * row_bytes + small);
+  float* u = reinterpret_cast<float*>(mem + 2 * row_bytes + 2 * small);
+  float* res = reinterpret_cast<float*>(mem + 2 * row_bytes + 3 * small);  // logprob or loss, entropy, stats
+  uint32_t* flag = reinterpret_cast<uint32_t*>(mem + 2 * row_bytes + 4 * small);
+  const Logits L{mem, nullptr, (unsigned long long)vocab, n, vocab};
+  const Teacher te{ids, u, kIds, 4, DET_DTYPE_F32, k};
+  const ScoreOut o{k ? nullptr : res, k ? nullptr : res + n, res + 2 * n, nullptr, nullptr, 0, flag};
+  float one[n], host[6 * n];
+  for (float& v : one) v = 1.0f;
+  cudaError_t e = cudaMemset(mem, 0, bytes);
+  if (e == cudaSuccess) e = cudaMemcpy(ones, one, sizeof(one), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess)
+    e = clusters_as<T, false, SELFTEST>(nullptr, L, ids, 4, k ? te : kNoTeacher, 1.0f, GradIn{nullptr, ones, nullptr},
+                                        mem + 2 * row_bytes + 5 * small, k ? res : nullptr, o, grad, vocab, 2);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(flags, flag, 4, cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess) e = cudaMemcpy(host, res, sizeof(host), cudaMemcpyDeviceToHost);
+  *all = *none = true;
+  auto look = [&](bool is_nan) {
+    *all &= is_nan;
+    *none &= !is_nan;
+  };
+  for (int i = 0; i < 6 * n; i++)
+    if (!k || i < n || i >= 2 * n) look(host[i] != host[i]);
+  for (size_t at = 0; at < (size_t)n * vocab && e == cudaSuccess;) {
+    uint16_t part[2048];
+    const size_t m = (size_t)n * vocab - at < 2048 ? (size_t)n * vocab - at : 2048;
+    e = cudaMemcpy(part, grad + at, 2 * m, cudaMemcpyDeviceToHost);
+    for (size_t i = 0; i < m; i++) look((part[i] & 0x7fff) > 0x7f80);
+    at += m;
+  }
+  cudaFree(mem);
+  return e;
+}
+
 static_assert(DET_SCORE_NONFINITE == (int)ERRF_CDF_NONFINITE && DET_SCORE_BAD_TOKEN == (int)ERRF_SYMBOL,
               "the flags are the session's error bits");
 }  // namespace det
@@ -1999,6 +2073,23 @@ static_assert(DET_SCORE_NONFINITE == (int)ERRF_CDF_NONFINITE && DET_SCORE_BAD_TO
 using namespace det;
 
 extern "C" {
+
+det_status det_step_timeout_selftest(int device) {
+  int cnt = 0;
+  if (cudaGetDeviceCount(&cnt) != cudaSuccess || cnt == 0) return DET_ERR_NO_DEVICE;
+  if (device < 0 || device >= cnt) return DET_ERR_INVALID_ARGUMENT;
+  if (cudaSetDevice(device) != cudaSuccess) return DET_ERR_CUDA;
+  bool reported = true;
+  for (int vocab : {5000, 40000})  // a block per row, and a cluster
+    for (int k : {0, 2}) {
+      bool all, none;
+      uint32_t flags = 0;
+      if (step_selftest_run<true>(vocab, k, &all, &none, &flags) != cudaSuccess) return DET_ERR_CUDA;
+      reported &= flags == DET_SCORE_TIMEOUT && all;
+      if (step_selftest_run<false>(vocab, k, &all, &none, &flags) != cudaSuccess || flags || !none) return DET_ERR_CUDA;
+    }
+  return reported ? DET_ERR_TIMEOUT : DET_OK;
+}
 
 size_t det_scores_workspace(int dtype, uint32_t n, uint32_t vocab, uint32_t top) {
   if (dtype < DET_DTYPE_F32 || dtype > DET_DTYPE_BF16 || vocab > kMaxVocab || n > DET_SCORE_MAX_ROWS) return 0;

@@ -14,8 +14,9 @@ a training step takes the gradient from the ``_step`` call, or from the
 
 What is wrong on the host side raises (``ValueError``, or :class:`DetError`
 with the library's status); what only the device sees (a NaN, a token outside
-the vocabulary) makes its row's results NaN, as ``include/detgpu.h`` lists.
-There is no CPU fallback.
+the vocabulary) makes its row's results NaN, as ``include/detgpu.h`` lists.  A
+``_step`` call whose kernel gave up a bounded wait, which is not expected, has
+NaN in all of its results.  There is no CPU fallback.
 """
 from __future__ import annotations
 

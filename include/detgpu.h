@@ -227,6 +227,13 @@ det_status det_tp_exchange_timeout_selftest(int device);
  * (expected result DET_ERR_TIMEOUT), then the same launch with every stage
  * copied must finish without an error (else DET_ERR_CUDA). */
 det_status det_q6k_pipeline_timeout_selftest(int device);
+/* Self-test of the bounded waits of the token score and distillation steps (no
+ * counterpart in the reference): on `device`, runs the step's kernels with one
+ * wait, in the middle of the rows, that nothing ends.  It gives up after 20 ms;
+ * the call's results then have to be NaN as a whole and DET_SCORE_TIMEOUT to be
+ * in its flags (expected result DET_ERR_TIMEOUT, DET_OK if not), and the same
+ * call with every wait ended must finish without either (else DET_ERR_CUDA). */
+det_status det_step_timeout_selftest(int device);
 /* Measured latency of one dependent rounded f32 add on `device`, in SM
  * clock cycles (one warp, 8,192 adds between two clock reads, best of
  * three): the floor of every ordered chain, e.g. the K adds of a Q4_K row.
@@ -323,8 +330,8 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  *   list entry: id < 0, u -inf not a valid entry; u NaN or +inf: as a bad id
  *   no valid entry in a list   loss 0 and gradient 0, whatever the logits
  *   an id listed twice         two terms of the loss; its gradient has both
- *   (a bounded wait of a step call's kernel ran out: DET_SCORE_TIMEOUT and NaN;
- *   it is not expected to)
+ *   (a bounded wait of a step call's kernel ran out: DET_SCORE_TIMEOUT, and all
+ *   of the call's results and gradients are NaN; it is not expected to)
  * A probability below 2^-123 of the row's largest counts as 0.
  *
  * Results are deterministic, and a row's are the same bits in whatever batch
