@@ -10,7 +10,8 @@ Each call runs on the current stream of the logits' device, does not
 synchronise, and may be captured into a CUDA graph.  Its results are new
 tensors (the gradient ``out`` where given).  Nothing is recorded by autograd:
 a training step takes the gradient from the ``_step`` call, or from the
-``_grad`` call in the backward of its own ``torch.autograd.Function``.
+``_grad`` call in the backward of its own ``torch.autograd.Function``.  Writing
+to ``out`` counts as a change in place.
 
 What is wrong on the host side raises (``ValueError``, or :class:`DetError`
 with the library's status); what only the device sees (a NaN, a token outside
@@ -85,6 +86,14 @@ def _grad_out(logits, out, n, vocab):
     return out, out.stride(0) if n > 1 else vocab
 
 
+def _given(out, grad):
+    # autograd is told that a caller's tensor was written to, so a backward
+    # that needs its old values is refused
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return grad
+
+
 def _lists(ids, teacher, logits, n):
     if ids.dim() != 2 or teacher.dim() != 2:
         raise ValueError("teacher_ids and teacher_logits must be [rows, entries]")
@@ -157,10 +166,10 @@ def token_scores_grad(logits, tokens, stats, grad_logprob=None, grad_entropy=Non
     ps = _on(stats, logits, "stats", (n, 4), (_F32,))
     gl = _vector(grad_logprob, logits, "grad_logprob", n)
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
-    out, out_ld = _grad_out(logits, out, n, vocab)
+    grad, grad_ld = _grad_out(logits, out, n, vocab)
     _call("det_token_scores_grad_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
-          _IDS[tokens.dtype], ps, gl, ge, out.data_ptr(), out_ld)
-    return out
+          _IDS[tokens.dtype], ps, gl, ge, grad.data_ptr(), grad_ld)
+    return _given(out, grad)
 
 
 def token_scores_step(logits, tokens, grad_logprob=None, grad_entropy=None, out=None):
@@ -171,13 +180,13 @@ def token_scores_step(logits, tokens, grad_logprob=None, grad_entropy=None, out=
     tok = _on(tokens, logits, "tokens", (n,), _IDS)
     gl = _vector(grad_logprob, logits, "grad_logprob", n)
     ge = _vector(grad_entropy, logits, "grad_entropy", n)
-    out, out_ld = _grad_out(logits, out, n, vocab)
+    grad, grad_ld = _grad_out(logits, out, n, vocab)
     logprob, entropy, stats = _new(logits, n), _new(logits, n), _new(logits, n, 4)
     work, size = _workspace(logits, _step_size(n, vocab, 1))
     _call("det_token_scores_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, tok,
-          _IDS[tokens.dtype], gl, ge, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld,
-          None, work.data_ptr(), size)
-    return TokenScores(logprob, entropy, stats), out
+          _IDS[tokens.dtype], gl, ge, logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), grad.data_ptr(),
+          grad_ld, None, work.data_ptr(), size)
+    return TokenScores(logprob, entropy, stats), _given(out, grad)
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) -> DistillLoss:
@@ -203,10 +212,10 @@ def distill_grad(logits, teacher_ids, teacher_logits, stats, grad_loss, temperat
     lists = _lists(teacher_ids, teacher_logits, logits, n)
     ps = _on(stats, logits, "stats", (n, 4), (_F32,))
     g = _vector(grad_loss, logits, "grad_loss", n)
-    out, out_ld = _grad_out(logits, out, n, vocab)
+    grad, grad_ld = _grad_out(logits, out, n, vocab)
     _call("det_distill_grad_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
-          temperature, ps, g, out.data_ptr(), out_ld)
-    return out
+          temperature, ps, g, grad.data_ptr(), grad_ld)
+    return _given(out, grad)
 
 
 def distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperature: float = 1.0, out=None):
@@ -215,9 +224,9 @@ def distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperature: fl
     n, vocab, ld = _logits(logits)
     lists = _lists(teacher_ids, teacher_logits, logits, n)
     g = _vector(grad_loss, logits, "grad_loss", n)
-    out, out_ld = _grad_out(logits, out, n, vocab)
+    grad, grad_ld = _grad_out(logits, out, n, vocab)
     loss, stats = _new(logits, n), _new(logits, n, 4)
     work, size = _workspace(logits, _step_size(n, vocab, lists[4]))
     _call("det_distill_step_device", logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, ld, *lists,
-          temperature, g, loss.data_ptr(), stats.data_ptr(), out.data_ptr(), out_ld, None, work.data_ptr(), size)
-    return DistillLoss(loss, stats), out
+          temperature, g, loss.data_ptr(), stats.data_ptr(), grad.data_ptr(), grad_ld, None, work.data_ptr(), size)
+    return DistillLoss(loss, stats), _given(out, grad)
