@@ -27,14 +27,13 @@
 
 #include <atomic>
 #include <cstring>
-#include <map>
-#include <mutex>
 #include <tuple>
 #include <type_traits>
 
 #include "../../include/detgpu.h"
 #include "dev_math.cuh"
 #include "internal.h"
+#include "known.h"
 
 namespace det {
 namespace {
@@ -1697,19 +1696,18 @@ cudaError_t by_dtype(int dtype, F f) {
 
 // Blocks of a kernel that the current device holds at once (cached: the answer
 // depends on the kernel and the launch alone).
-int resident_blocks(const void* kern, int threads, size_t smem) {
+cudaError_t resident_blocks(const void* kern, int threads, size_t smem, int* out) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
-  static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int, size_t>, int> known;
-  std::lock_guard<std::mutex> lock(mu);
-  int& n = known[{kern, dev, threads, smem}];
-  if (n > 0) return n;
-  int per = 0, sms = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, smem) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    cudaGetLastError();
-  return n = per * sms > 0 ? per * sms : 1;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  static Known<std::tuple<const void*, int, int, size_t>, int> known;
+  return known.get({kern, dev, threads, smem}, out, [&](int* n) {
+    int per = 0, sms = 0;
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, smem);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) cudaGetLastError();
+    *n = per * sms;
+    return e == cudaSuccess && *n <= 0 ? cudaErrorInvalidConfiguration : e;
+  });
 }
 
 // How a kernel with a warp per segment takes rows of nseg segments: clusters of
@@ -1729,11 +1727,8 @@ cudaError_t cluster_plan(const void* kern, int nseg, size_t stage, ClusterPlan* 
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return e;
   if (cudaError_t e = raise_smem_cap(kern, kWarps * stage)) return e;
-  static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int>, ClusterPlan> known;
-  std::lock_guard<std::mutex> lock(mu);
-  ClusterPlan& best = known[{kern, dev, nseg}];
-  if (best.fit == 0) {
+  static Known<std::tuple<const void*, int, int>, ClusterPlan> known;
+  return known.get({kern, dev, nseg}, out, [&](ClusterPlan* best) {
     // clusters above 8 blocks have to be allowed
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
     ClusterPlan plans[kWarps];
@@ -1744,7 +1739,7 @@ cudaError_t cluster_plan(const void* kern, int nseg, size_t stage, ClusterPlan* 
       p.warps = (nseg + p.c - 1) / p.c;
       if (p.c > 16 || p.warps != w) continue;
       if (p.c == 1) {
-        p.fit = resident_blocks(kern, 32 * w, w * stage);
+        if (cudaError_t e = resident_blocks(kern, 32 * w, w * stage, &p.fit)) return e;
       } else {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)p.c);
@@ -1756,20 +1751,18 @@ cudaError_t cluster_plan(const void* kern, int nseg, size_t stage, ClusterPlan* 
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&p.fit, kern, &cfg) != cudaSuccess) {
+        if (cudaError_t e = cudaOccupancyMaxActiveClusters(&p.fit, kern, &cfg)) {
           cudaGetLastError();
-          continue;
+          return e;
         }
       }
       plans[n++] = p;
       most = most < p.fit ? p.fit : most;
     }
-    for (int i = 0; i < n && best.fit == 0; i++)
-      if (100 * plans[i].fit >= 93 * most) best = plans[i];
-    if (best.fit == 0) return cudaErrorInvalidConfiguration;
-  }
-  *out = best;
-  return cudaSuccess;
+    for (int i = 0; i < n && best->fit == 0; i++)
+      if (100 * plans[i].fit >= 93 * most) *best = plans[i];
+    return best->fit > 0 ? cudaSuccess : cudaErrorInvalidConfiguration;
+  });
 }
 // launches `clusters` clusters of c blocks, with programmatic stream
 // serialization
@@ -1827,7 +1820,8 @@ cudaError_t forward_as(cudaStream_t s, const Logits& L, const void* tokens, int 
   const size_t smem = kSegWarps * kStageBytes<T>;
   if (cudaError_t e = raise_smem_cap((const void*)segments, smem)) return e;
   const long long nseg = (L.vocab + kSeg - 1) / kSeg, blocks = (L.n * nseg + kSegWarps - 1) / kSegWarps;
-  const int fit = resident_blocks((const void*)segments, kSegThreads, smem);
+  int fit = 0;
+  if (cudaError_t e = resident_blocks((const void*)segments, kSegThreads, smem, &fit)) return e;
   Workspace ws;
   ws.seg = static_cast<float4*>(workspace);
   ws.gmax = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + align256(L.n * nseg * sizeof(float4)));
@@ -1854,8 +1848,9 @@ cudaError_t grad_as(cudaStream_t s, const Logits& L, const void* tokens, int id_
   const int nvec = (L.vocab + VEC - 1) / VEC + 1;  // one more where a row starts inside a vector
   // Runs per warp, up to 8: the waves of blocks, times a block's runs and what
   // it costs beside them (half a run's time; a list takes about two)
-  const int step = kThreads * kGradUnroll, fit = resident_blocks((const void*)grad_kernel<T, ENTROPY>, kThreads, 0);
-  int per = step;
+  const int step = kThreads * kGradUnroll;
+  int per = step, fit = 0;
+  if (cudaError_t e = resident_blocks((const void*)grad_kernel<T, ENTROPY>, kThreads, 0, &fit)) return e;
   float least = 0.0f;
   for (int runs = 1; runs <= 8; runs++) {
     const long long all = (long long)L.n * ((nvec + runs * step - 1) / (runs * step));
