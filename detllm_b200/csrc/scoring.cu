@@ -94,7 +94,8 @@ DI float max_nan(float a, float b) {  // NaN if either is
 // entry of a row with its two sums, against 19 for a degree-5 polynomial on
 // |f| <= 1/2: issue slots (two for a packed operation) bound the passes over
 // 16-bit logits.
-// Within 7.1 * 2^-24 of 2^y where that is 2^-122 or more, and 0 below 2^-123.
+// Within 7.1 * 2^-24 of 2^y from y = -123.953 on, and 0 below that: there the
+// entry times 2^k is no normal number any more.
 // NaN gives an unspecified number: callers keep y, which stays NaN, beside it.
 constexpr float kYLow = -127.5f;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147182f;

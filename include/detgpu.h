@@ -332,7 +332,7 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  *   an id listed twice         two terms of the loss; its gradient has both
  *   (a bounded wait of a step call's kernel ran out: DET_SCORE_TIMEOUT, and all
  *   of the call's results and gradients are NaN; it is not expected to)
- * A probability below 2^-123 of the row's largest counts as 0.
+ * A probability below 2^-122 of the row's largest may count as 0.
  *
  * Results are deterministic, and a row's are the same bits in whatever batch
  * or stride it is (the order of its sums depends on the vocabulary and the
