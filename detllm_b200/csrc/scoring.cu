@@ -271,10 +271,11 @@ DI uint4 load16(const uint4* p) {
   if constexpr (RO) return __ldg(p);
   else return *p;
 }
-// The vector at entry `at` of a row (RO: that nothing writes while the kernel
-// runs); what is past the row's end is -inf.  Only 16-byte granules that lie in
-// the row as a whole are loaded as such: a row that starts `mis` entries into a
-// granule takes two of them.
+// The vector at entry `at` of a row (RO: that nothing writes from the kernel's
+// launch on, so not in a kernel whose own pdl_wait() waits for the row); what is
+// past the row's end is -inf.  Only 16-byte granules that lie in the row as a
+// whole are loaded as such: a row that starts `mis` entries into a granule takes
+// two of them.
 template <typename T, bool RO = true>
 DI uint4 row_vec(const T* row, int at, int V, int mis) {
   constexpr int VEC = Seg<T>::VEC;
@@ -1620,7 +1621,7 @@ __global__ void __launch_bounds__(32 * kSmallSegs)
   float v[MODE == kGrad ? kPerLane : 1], m_seg = -INFINITY;
   if (g < nseg) {
 #pragma unroll
-    for (int i = 0; i < G::NV; i++) raw[i] = row_vec<T, MODE == kScores>(x, g * kSeg + (32 * i + l) * G::VEC, V, mis);
+    for (int i = 0; i < G::NV; i++) raw[i] = row_vec<T, false>(x, g * kSeg + (32 * i + l) * G::VEC, V, mis);
     Range<T> range;
 #pragma unroll
     for (int i = 0; i < G::NV; i++) range.take(raw[i]);
