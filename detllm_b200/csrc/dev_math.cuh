@@ -405,9 +405,14 @@ DI int q6k_quant(const uint8_t* body, int index) {
 // may start while its predecessor in the stream is still running.
 // pdl_wait() blocks until the predecessor grid has completed and its memory
 // writes are visible (it returns at once for a plain launch); every kernel
-// calls it before it reads or writes anything another kernel touches.
-// pdl_trigger() then lets the successor begin launching.  Only reads of
-// constant data (weights) may come before pdl_wait().
+// calls it, in all of its blocks, before it reads or writes anything another
+// kernel touches.  pdl_trigger() then lets the successor begin launching.  Only
+// reads of constant data (weights) may come before pdl_wait(), and what the
+// launch in front of it, in the same call, makes safe: where that kernel calls
+// pdl_wait() in all of its blocks before any of them triggers or ends, all that
+// ran before the call is complete by the time the successor starts, so the
+// successor may read the call's inputs, and nothing that the call itself writes,
+// before its own pdl_wait() (the second and third kernels in scoring.cu).
 DI void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 DI void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 DI void pdl_enter() {

@@ -91,7 +91,8 @@ struct Launch {
 
 // Launch `kern` on L.stream, with programmatic stream serialization when
 // L.pdl (the kernel may then start before its predecessor finishes; every
-// kernel calls pdl_wait() first, see dev_math.cuh).  DETGPU_NO_PDL=1 turns
+// kernel calls pdl_wait() before it touches what that one writes, see
+// dev_math.cuh for what may come first).  DETGPU_NO_PDL=1 turns
 // the attribute off everywhere.
 bool pdl_enabled();
 template <typename... KArgs, typename... Args>

@@ -998,7 +998,8 @@ __global__ void __launch_bounds__(kRowThreads, 7)
   const T* x = static_cast<const T*>(L.x) + (size_t)(L.rows ? L.rows[row] : row) * L.ld;
   const float c = fdiv(kLog2e, temp), nan = __int_as_float(0x7fffffff);
   const uint32_t table = kExpTable[threadIdx.x & 31];
-  // what does not depend on the sums, while they are being taken
+  // what does not depend on the sums, while they are being taken: inputs of the
+  // call, which are complete, as segments_kernel waits before it triggers
   ListEntry e;
   float z = 0.0f;
   double logq = 0.0;
@@ -1312,6 +1313,8 @@ __global__ void __launch_bounds__(kThreads)
     step_gather_kernel(Logits L, const void* tokens, int id_bytes, Teacher te, float temp, GradIn in, StepWork ws,
                        uint32_t first) {
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), l = threadIdx.x & 31, V = L.vocab;
+  // Every block waits, and none triggers before it does (none triggers at all):
+  // the next two kernels read the call's inputs before their own waits.
   pdl_wait();
   if (row >= L.n) return;
   if (row == 0 && l == 0) ws.ticket[0] = first, ws.ticket[1] = 0;
@@ -1450,6 +1453,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   void* stage = dyn + w * kStageBytes<T>;
   auto at_row = [&](int r) { return static_cast<const T*>(L.x) + (size_t)r * L.ld; };
   int row = blockIdx.x / size, next = row + clusters;
+  // before pdl_wait(): the logits are complete, as step_gather_kernel has waited
+  // in all blocks, and only this kernel writes over them.  The kernel after this
+  // one reads inputs alone before its wait, so it may be launched already.
   if (active) stage_issue<T>(stage, at_row(row), g, V);
   pdl_trigger();
   const float c = fdiv(kLog2e, temp);
@@ -1542,6 +1548,7 @@ __global__ void __launch_bounds__(kRowThreads)
   long long t = -1;
   int id, own;
   float share = 0.0f;
+  // the call's inputs, complete since step_gather_kernel waited
   if (loss) {
     e = teacher_entry(te, row, V, c, table, one, list);
     logq = list_logq(e, temp);
