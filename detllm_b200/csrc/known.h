@@ -3,11 +3,13 @@
 
 #include <map>
 #include <mutex>
+#include <new>
 
 namespace det {
 
 // get() gives what ask(&value) gave for the key.  Only an answer is kept: a
-// query that fails hands its error on, and the next call asks again.
+// query that fails hands its error on, and the next call asks again; so it does
+// where there is no memory to keep the answer.
 template <typename Key, typename Value>
 class Known {
  public:
@@ -21,7 +23,12 @@ class Known {
     }
     Value v{};
     const auto error = ask(&v);
-    if (error == decltype(ask(out)){}) known_[key] = *out = v;
+    if (error != decltype(ask(out)){}) return error;
+    *out = v;
+    try {
+      known_.emplace(key, v);
+    } catch (const std::bad_alloc&) {
+    }
     return error;
   }
 

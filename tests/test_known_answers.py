@@ -1,5 +1,5 @@
 """The library's cache of what it asks the device (known.h): an answer is kept,
-a failed query is reported and asked again.  Compiled and run on the host, with
+a failed query is reported and asked again, and no exception leaves it.  Compiled and run on the host, with
 a query that fails where the device's would."""
 import os
 import subprocess
@@ -8,8 +8,18 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 PROGRAM = r"""
 #include <cstdio>
+#include <cstdlib>
+#include <new>
 #include <utility>
 #include "known.h"
+
+static bool memory = true;
+void* operator new(std::size_t n) {
+  if (!memory) throw std::bad_alloc();
+  return std::malloc(n);
+}
+void operator delete(void* p) noexcept { std::free(p); }
+void operator delete(void* p, std::size_t) noexcept { std::free(p); }
 
 enum Error { kNone = 0, kBusy = 7 };
 
@@ -25,6 +35,11 @@ int main() {
   value = 0;
   if (known.get({1, 2}, &value, never) != kNone || value != 42 || asked != 3) return 4;
   if (known.get({2, 1}, &value, fails) != kBusy || value != 42 || asked != 4) return 5;
+  // no memory to keep it: handed out all the same, and asked again
+  memory = false;
+  value = 0;
+  for (int i = 0; i < 2; i++)
+    if (known.get({3, 3}, &value, answer) != kNone || value != 42 || asked != 5 + i) return 6;
   std::puts("kept");
   return 0;
 }
