@@ -332,7 +332,11 @@ det_status det_symbol_ranges_noalloc(const float* logits, uint32_t n, uint32_t v
  *   an id listed twice         two terms of the loss; its gradient has both
  *   (a bounded wait of a step call's kernel ran out: DET_SCORE_TIMEOUT, and all
  *   of the call's results and gradients are NaN; it is not expected to)
- * A probability below 2^-122 of the row's largest may count as 0.
+ * Where several of these meet: a row that is not a number comes before its
+ * token, and a bad id before the rest of its list; a list without a valid entry
+ * comes before its row; a row of nothing but -inf has a gradient of 0 whatever
+ * its token or list.  A token is looked at where logprob or its gradient is asked
+ * for.  A probability below 2^-122 of the row's largest may count as 0.
  *
  * Results are deterministic, and a row's are the same bits in whatever batch
  * or stride it is (the order of its sums depends on the vocabulary and the
