@@ -787,7 +787,9 @@ DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int
   }
   __syncthreads();
   // a value that at least k of them reach: the lower end of the bin, of 256
-  // between the smallest and the largest, that the k-th largest is in
+  // between the smallest and the largest, that the k-th largest is in.  The bins
+  // are equally wide in the ordered integers: with a maximum of 0 or less among
+  // them they span exponents down to 0, and many groups reach the floor.
   uint32_t floor = 0;
   if (ng > k) {
     lo = sh.lo;
@@ -848,9 +850,11 @@ DI void top_list(const T* __restrict__ x, int V, int mis, const float* gmax, int
   }
   __syncthreads();
   if (!few || sh.count > kCand) {
-    // too many groups or entries reach the floor (ties, or a row in order): group by group in the order of their indices, cutting the list
-    // down as it fills, which raises the floor and passes over the groups that
-    // cannot add to it
+    // too many groups or entries reach the floor (ties, a row in order, or a wide
+    // bin): group by group in the order of their indices, cutting the list down
+    // as it fills, which raises the floor and passes over the groups that cannot
+    // add to it.  1,024 rows of 128,256 f32, top 20: 376 us with the last 256
+    // entries masked out, 126 without.
     __syncthreads();
     if (tid == 0) sh.count = 0;
     __syncthreads();
@@ -1296,7 +1300,7 @@ DI void store_segment(T* y, int g, int V, int my, F vec) {
 // have two places and two mbarriers; a warp sends the row after next only when
 // it has the next row's sums, which every warp sent after it read the row's.
 //
-// 1,024 rows of 128,256 bf16 logits: 148 us, memory read and written once in 81
+// 1,024 rows of 128,256 bf16 logits: 147 us, memory read and written once in 81
 // us; 177 us with a cluster barrier per row, 182 us as sums and gradient over
 // memory, 190 us and more as tasks that a persistent grid draws, sums a chunk
 // of rows ahead of gradients that find their logits in the L2 cache (two passes'
@@ -1892,8 +1896,8 @@ size_t step_workspace_bytes(size_t n, int k) {
 }
 // the three kernels; `most`: clusters at most
 template <typename T, bool ENTROPY, bool SELFTEST = false>
-cudaError_t clusters_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te, float temp,
-                        const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
+cudaError_t clusters_as(cudaStream_t s, const Logits& L, const void* tokens, int id_bytes, const Teacher& te,
+                        float temp, const GradIn& in, void* workspace, float* loss, const ScoreOut& o, void* out,
                         unsigned long long out_ld, int most) {
   const size_t n = L.n, k = te.k ? te.k : 1;
   uint8_t* at = static_cast<uint8_t*>(workspace);
